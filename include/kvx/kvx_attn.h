@@ -1,0 +1,81 @@
+/*
+ * kvx — C ABI of the operators on what the cache rows hold (libkvx.so): rows
+ * in 8 bits, and attention over the hot buffer.  No counterpart in the
+ * reference, which moves rows as bytes.  Conventions as in kvx/kvx.h: device
+ * addresses and sizes as plain integers, asynchronous launches on `stream`
+ * (0 = the null stream), a nonzero return is an error whose message
+ * kvx_last_error() gives.
+ *
+ * A row holds kv_lora_rank values that every query head uses as keys and as
+ * values, then qk_rope values used as keys only (512 and 64: the sizes the
+ * kernels are built for), in one of three forms:
+ *
+ *   KVX_QUANT_NONE    576 16-bit values                            1152 bytes
+ *   KVX_QUANT_LATENT  512 codes, 64 16-bit values, 16 scale bytes   768 bytes
+ *   KVX_QUANT_ROW     576 codes, 18 scale bytes                     640 bytes
+ *
+ * the 8-bit forms padded with zeros.  Codes are e4m3 (no infinities), one
+ * scale for each 32 of them in order: the byte e + 127 of the power of two
+ * 2^e, the smallest one for which the largest finite magnitude of the group
+ * is at most 448 * 2^e (e >= -127; a group of zeros has -127).  A value is
+ * rounded to the nearest code (ties to even); a NaN stays one, an infinity
+ * becomes the largest code of its sign.
+ *
+ * Rows are named as in the imports: request b's slot s is hot row
+ * b * req_stride_rows + s.  A negative slot names no row; so does one whose
+ * row is not below hot_rows, which besides sets the tail-slot word
+ * (kvx_read_overflow) to KVX_OVERFLOW_ROW.
+ */
+#ifndef KVX_KVX_ATTN_H
+#define KVX_KVX_ATTN_H
+
+#include <stdint.h>
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+enum { KVX_DTYPE_BF16 = 0, KVX_DTYPE_FP16 = 1, KVX_DTYPE_FP32 = 2 };
+enum { KVX_QUANT_NONE = 0, KVX_QUANT_LATENT = 1, KVX_QUANT_ROW = 2 };
+
+#define KVX_OVERFLOW_ROW 0x524F57ull
+
+/* Write num_reqs * rows_per_req rows of 16-bit values (dtype; row i at src +
+ * i * src_stride_bytes) into hot rows of form quant (LATENT or ROW).  slots:
+ * int32 [num_reqs, rows_per_req] on the device; 0: row i goes to hot row i
+ * (which all have to be below hot_rows).  Rows without a slot are left out.
+ * Two rows of one call that name the same slot leave it undefined. */
+int kvx_quantize_rows(uint64_t src, uint64_t src_stride_bytes, uint64_t hot_row_base, uint64_t hot_rows,
+                      uint64_t slots, uint32_t num_reqs, uint32_t rows_per_req, uint64_t req_stride_rows,
+                      uint32_t kv_lora_rank, uint32_t qk_rope, uint32_t dtype, uint32_t quant, uint64_t stream);
+
+/* Read such rows back: row i of dst (out_dtype, kv_lora_rank + qk_rope values,
+ * contiguous) gets the values of the i-th slot's row rounded to out_dtype, zeros where there is none. */
+int kvx_dequantize_rows(uint64_t hot_row_base, uint64_t hot_rows, uint64_t slots, uint32_t num_reqs,
+                        uint32_t rows_per_req, uint64_t req_stride_rows, uint64_t dst, uint32_t kv_lora_rank,
+                        uint32_t qk_rope, uint32_t dtype, uint32_t quant, uint32_t out_dtype, uint64_t stream);
+
+/* Attention of each request's drafted tokens over its selected slots and over
+ * the drafted tokens' own rows.  Query (b, t, h), 576 16-bit values (dtype) at
+ * q + b * q_stride_b + t * q_stride_t + h * q_stride_h (bytes), sees the keys
+ *   - slots[b][k], k < top_k (int32 [num_reqs, top_k]), and
+ *   - draft_slots[b][j], j < draft (int32 [num_reqs, draft], or 0: none), where
+ *     bit j of tree_mask[b][t] is set (uint64 [num_reqs, draft], or 0: j <= t)
+ * that name a row.  With s = softmax_scale * q.k over all 576 values:
+ *   lse[b][t][h] = ln sum exp s                        (float32; 0: not written)
+ *   out[b][t][h] = sum exp(s - lse) * first 512 values  (dtype, contiguous)
+ * and zeros with lse -inf where a query sees no key.  A key listed twice
+ * counts twice.  What rows hold that a query does not see has no effect on it,
+ * NaN and infinities included.  draft <= 64, heads <= 1024.  Scores, sums and the output
+ * are accumulated in 32 bits, the weights exp(s - max) rounded to dtype. */
+int kvx_tree_attention(uint64_t q, uint64_t q_stride_b, uint64_t q_stride_t, uint64_t q_stride_h,
+                       uint64_t hot_row_base, uint64_t hot_rows, uint64_t slots, uint64_t draft_slots,
+                       uint64_t tree_mask, uint64_t out, uint64_t lse, uint32_t num_reqs, uint32_t draft,
+                       uint32_t heads, uint32_t top_k, uint64_t req_stride_rows, float softmax_scale,
+                       uint32_t kv_lora_rank, uint32_t qk_rope, uint32_t dtype, uint32_t quant, uint64_t stream);
+
+#ifdef __cplusplus
+}
+#endif
+
+#endif /* KVX_KVX_ATTN_H */

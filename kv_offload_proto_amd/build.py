@@ -1,6 +1,6 @@
 """Build the native parts of kv_offload_proto_amd in-tree.
 
-* ``kvops_ext/libkvx.so`` -- the gfx950 kernels and the C ABI (include/kvx/kvx.h),
+* ``kvops_ext/libkvx.so`` -- the gfx950 kernels and the C ABI (include/kvx/kvx.h, kvx_attn.h),
   compiled by hipcc for ``--offload-arch=gfx950``.
 * ``kvops_ext/_kvops*.so`` -- the pybind11 module with the reference's
   ``kvops_ext._kvops`` surface, linked against libkvx.so (rpath $ORIGIN).
@@ -22,7 +22,7 @@ OUT = os.path.join(HERE, "kvops_ext")
 INCLUDE = os.path.join(ROOT, "include")
 
 HIP_SOURCES = ["sieve.hip", "sieve_fast.hip", "sieve_wave.hip", "sieve_batch.hip", "sieve_table.hip", "rows.hip",
-               "kvx_host.hip"]
+               "quant_rows.hip", "attn.hip", "kvx_host.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 HIP_FLAGS = [

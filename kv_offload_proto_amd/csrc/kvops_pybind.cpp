@@ -11,6 +11,7 @@
 #include <vector>
 
 #include "kvx/kvx.h"
+#include "kvx/kvx_attn.h"
 #include "kvx_admit.h"
 
 namespace py = pybind11;
@@ -257,6 +258,44 @@ PYBIND11_MODULE(_kvops, m)
         py::arg("stream") = 0);
     m.def("last_sieve_variant", []() { return kvx_last_sieve_variant(); });
     m.def("sieve_force_variant", [](int variant) { Check(kvx_sieve_force_variant(variant)); }, py::arg("variant"));
+    m.def(
+        "quantize_rows",
+        [](uint64_t src, uint64_t src_stride_bytes, uint64_t hot_row_base, uint64_t hot_rows, uint64_t slots,
+           uint32_t num_reqs, uint32_t rows_per_req, uint64_t req_stride_rows, uint32_t kv_lora_rank, uint32_t qk_rope,
+           uint32_t dtype, uint32_t quant, uint64_t stream) {
+            Check(kvx_quantize_rows(src, src_stride_bytes, hot_row_base, hot_rows, slots, num_reqs, rows_per_req,
+                                    req_stride_rows, kv_lora_rank, qk_rope, dtype, quant, stream));
+        },
+        py::arg("src"), py::arg("src_stride_bytes"), py::arg("hot_row_base"), py::arg("hot_rows"), py::arg("slots"),
+        py::arg("num_reqs"), py::arg("rows_per_req"), py::arg("req_stride_rows"), py::arg("kv_lora_rank"),
+        py::arg("qk_rope"), py::arg("dtype"), py::arg("quant"), py::arg("stream") = 0);
+    m.def(
+        "dequantize_rows",
+        [](uint64_t hot_row_base, uint64_t hot_rows, uint64_t slots, uint32_t num_reqs, uint32_t rows_per_req,
+           uint64_t req_stride_rows, uint64_t dst, uint32_t kv_lora_rank, uint32_t qk_rope, uint32_t dtype,
+           uint32_t quant, uint32_t out_dtype, uint64_t stream) {
+            Check(kvx_dequantize_rows(hot_row_base, hot_rows, slots, num_reqs, rows_per_req, req_stride_rows, dst,
+                                      kv_lora_rank, qk_rope, dtype, quant, out_dtype, stream));
+        },
+        py::arg("hot_row_base"), py::arg("hot_rows"), py::arg("slots"), py::arg("num_reqs"), py::arg("rows_per_req"),
+        py::arg("req_stride_rows"), py::arg("dst"), py::arg("kv_lora_rank"), py::arg("qk_rope"), py::arg("dtype"),
+        py::arg("quant"), py::arg("out_dtype"), py::arg("stream") = 0);
+    m.def(
+        "tree_attention",
+        [](uint64_t q, uint64_t q_stride_b, uint64_t q_stride_t, uint64_t q_stride_h, uint64_t hot_row_base,
+           uint64_t hot_rows, uint64_t slots, uint64_t draft_slots, uint64_t tree_mask, uint64_t out, uint64_t lse,
+           uint32_t num_reqs, uint32_t draft, uint32_t heads, uint32_t top_k, uint64_t req_stride_rows,
+           float softmax_scale, uint32_t kv_lora_rank, uint32_t qk_rope, uint32_t dtype, uint32_t quant,
+           uint64_t stream) {
+            Check(kvx_tree_attention(q, q_stride_b, q_stride_t, q_stride_h, hot_row_base, hot_rows, slots, draft_slots,
+                                     tree_mask, out, lse, num_reqs, draft, heads, top_k, req_stride_rows,
+                                     softmax_scale, kv_lora_rank, qk_rope, dtype, quant, stream));
+        },
+        py::arg("q"), py::arg("q_stride_b"), py::arg("q_stride_t"), py::arg("q_stride_h"), py::arg("hot_row_base"),
+        py::arg("hot_rows"), py::arg("slots"), py::arg("draft_slots"), py::arg("tree_mask"), py::arg("out"),
+        py::arg("lse"), py::arg("num_reqs"), py::arg("draft"), py::arg("heads"), py::arg("top_k"),
+        py::arg("req_stride_rows"), py::arg("softmax_scale"), py::arg("kv_lora_rank"), py::arg("qk_rope"),
+        py::arg("dtype"), py::arg("quant"), py::arg("stream") = 0);
     m.def(
         "stream_copy",
         [](uint64_t dst, uint64_t src, uint64_t nbytes, uint64_t stream) {

@@ -26,6 +26,7 @@
 #include "kvx/kvx.h"
 #include "kvx_admit.h"
 #include "kvx_internal.h"
+#include "row_format.h"
 
 namespace {
 
@@ -488,6 +489,38 @@ void DoExportRows(const uint64_t *segBases, bool fused, uint32_t layer_id, uint3
         ClearStatusWords(status, my_node, a.statusWords);
     }
     hipCheck(kvx::launch_export_rows(a, segBases, scr, AsStream(stream)), "export_rows launch");
+}
+
+void CheckRowForm(const char *what, uint32_t latent, uint32_t rope, uint32_t dtype, uint32_t quant, bool codes)
+{
+    const std::string name(what);
+    if (latent != static_cast<uint32_t>(kvx::kLatent) || rope != static_cast<uint32_t>(kvx::kRope)) {
+        throw Error(name + ": rows of kv_lora_rank 512 and qk_rope 64 are supported, got " + std::to_string(latent) +
+                    " and " + std::to_string(rope));
+    }
+    if (dtype > KVX_DTYPE_FP16) throw Error(name + ": dtype must be bf16 or fp16");
+    if (quant > KVX_QUANT_ROW) throw Error(name + ": unknown row form");
+    if (codes && quant == KVX_QUANT_NONE) throw Error(name + ": rows of 16-bit values hold no codes");
+}
+
+kvx::RowCopyArgs RowCopy(const char *what, uint64_t rows16, uint64_t rowStride, uint64_t hot, uint64_t hotRows,
+                         uint64_t slots, uint32_t numReqs, uint32_t rowsPerReq, uint64_t reqStride)
+{
+    kvx::RowCopyArgs a{};
+    a.rows16 = rows16;
+    a.rowStride = rowStride;
+    a.hot = hot;
+    a.hotRows = hotRows;
+    a.slots = slots;
+    a.reqStride = reqStride;
+    a.rows = static_cast<uint64_t>(numReqs) * rowsPerReq;
+    a.perReq = rowsPerReq;
+    a.overflowSlot = reinterpret_cast<uint64_t>(g.overflow);
+    const std::string name(what);
+    if (a.rows >= 1ull << 31) throw Error(name + ": num_reqs * rows_per_req must be below 2^31");
+    if (slots == 0 && a.rows > hotRows) throw Error(name + ": more rows than hot_rows and no slots");
+    if (a.rows != 0 && (rows16 == 0 || hot == 0)) throw Error(name + ": the rows must be device addresses");
+    return a;
 }
 
 // Node masks for the memory-policy system calls: up to 1024 nodes (the
@@ -1116,6 +1149,89 @@ int kvx_close(void)
             g.noAllocPending[d] = false;
         }
         g.inited = false;
+    });
+}
+
+int kvx_quantize_rows(uint64_t src, uint64_t src_stride_bytes, uint64_t hot_row_base, uint64_t hot_rows,
+                      uint64_t slots, uint32_t num_reqs, uint32_t rows_per_req, uint64_t req_stride_rows,
+                      uint32_t kv_lora_rank, uint32_t qk_rope, uint32_t dtype, uint32_t quant, uint64_t stream)
+{
+    return Guarded([&] {
+        EnsureInited();
+        CheckRowForm("quantize_rows", kv_lora_rank, qk_rope, dtype, quant, true);
+        CheckAligned16(src, "quantize_rows: src");
+        CheckAligned16(hot_row_base, "quantize_rows: hot_row_base");
+        if (src_stride_bytes % 16 != 0) throw Error("quantize_rows: src_stride_bytes must be a multiple of 16");
+        const kvx::RowCopyArgs a = RowCopy("quantize_rows", src, src_stride_bytes, hot_row_base, hot_rows, slots,
+                                           num_reqs, rows_per_req, req_stride_rows);
+        if (a.rows == 0) return;
+        hipCheck(kvx::launch_quantize_rows(a, dtype, quant, AsStream(stream)), "quantize_rows launch");
+    });
+}
+
+int kvx_dequantize_rows(uint64_t hot_row_base, uint64_t hot_rows, uint64_t slots, uint32_t num_reqs,
+                        uint32_t rows_per_req, uint64_t req_stride_rows, uint64_t dst, uint32_t kv_lora_rank,
+                        uint32_t qk_rope, uint32_t dtype, uint32_t quant, uint32_t out_dtype, uint64_t stream)
+{
+    return Guarded([&] {
+        EnsureInited();
+        CheckRowForm("dequantize_rows", kv_lora_rank, qk_rope, dtype, quant, true);
+        if (out_dtype > KVX_DTYPE_FP32) throw Error("dequantize_rows: unknown out_dtype");
+        CheckAligned16(hot_row_base, "dequantize_rows: hot_row_base");
+        CheckAligned16(dst, "dequantize_rows: dst");
+        const kvx::RowCopyArgs a = RowCopy("dequantize_rows", dst, 0, hot_row_base, hot_rows, slots, num_reqs,
+                                           rows_per_req, req_stride_rows);
+        if (a.rows == 0) return;
+        hipCheck(kvx::launch_dequantize_rows(a, dtype, quant, out_dtype, AsStream(stream)), "dequantize_rows launch");
+    });
+}
+
+int kvx_tree_attention(uint64_t q, uint64_t q_stride_b, uint64_t q_stride_t, uint64_t q_stride_h,
+                       uint64_t hot_row_base, uint64_t hot_rows, uint64_t slots, uint64_t draft_slots,
+                       uint64_t tree_mask, uint64_t out, uint64_t lse, uint32_t num_reqs, uint32_t draft,
+                       uint32_t heads, uint32_t top_k, uint64_t req_stride_rows, float softmax_scale,
+                       uint32_t kv_lora_rank, uint32_t qk_rope, uint32_t dtype, uint32_t quant, uint64_t stream)
+{
+    return Guarded([&] {
+        EnsureInited();
+        CheckRowForm("tree_attention", kv_lora_rank, qk_rope, dtype, quant, false);
+        if (num_reqs == 0 || draft == 0 || heads == 0) return;
+        if (draft > 64) throw Error("tree_attention: draft must be <= 64");
+        if (heads > 1024) throw Error("tree_attention: heads must be <= 1024");
+        if (top_k > (1u << 30)) throw Error("tree_attention: top_k must be <= 2^30");
+        CheckAligned16(q, "tree_attention: q");
+        CheckAligned16(hot_row_base, "tree_attention: hot_row_base");
+        CheckAligned16(out, "tree_attention: out");
+        if ((q_stride_b | q_stride_t | q_stride_h) % 16 != 0) {
+            throw Error("tree_attention: the strides of q must be multiples of 16 bytes");
+        }
+        if (q == 0 || out == 0) throw Error("tree_attention: q and out must be device addresses");
+        if ((top_k != 0 && slots == 0) || (hot_rows != 0 && hot_row_base == 0)) {
+            throw Error("tree_attention: slots and hot_row_base must be device addresses");
+        }
+        kvx::AttnArgs a{};
+        a.q = q;
+        a.qStrideB = q_stride_b;
+        a.qStrideT = q_stride_t;
+        a.qStrideH = q_stride_h;
+        a.hot = hot_row_base;
+        a.hotRows = hot_rows;
+        a.reqStride = req_stride_rows;
+        a.slots = slots;
+        a.draftSlots = draft_slots;
+        a.treeMask = tree_mask;
+        a.out = out;
+        a.lse = lse;
+        a.reqs = num_reqs;
+        a.draft = draft;
+        a.heads = heads;
+        a.topK = top_k;
+        a.scaleLog2 = softmax_scale * 1.4426950408889634f;
+        a.overflowSlot = reinterpret_cast<uint64_t>(g.overflow);
+        if (static_cast<uint64_t>(num_reqs) * draft * heads >= 1ull << 31) {
+            throw Error("tree_attention: num_reqs * draft * heads must be below 2^31");
+        }
+        hipCheck(kvx::launch_tree_attention(a, dtype, quant, AsStream(stream)), "tree_attention launch");
     });
 }
 

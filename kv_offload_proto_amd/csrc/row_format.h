@@ -1,0 +1,71 @@
+// Layout of the cache rows as the kernels read and write them (the forms of
+// kvx/kvx_attn.h), and the arguments of the launches on them.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "kvx/kvx_attn.h"
+
+namespace kvx {
+
+constexpr int kLatent = 512;
+constexpr int kRope = 64;
+constexpr int kDim = kLatent + kRope;
+constexpr int kGroup = 32;   // values that share a scale
+
+template <int QUANT>
+struct RowForm {
+    static constexpr int codes = QUANT == KVX_QUANT_NONE ? 0 : (QUANT == KVX_QUANT_LATENT ? kLatent : kDim);
+    static constexpr int raw = kDim - codes;             // values kept in 16 bits, behind the codes
+    static constexpr int scaleAt = codes + 2 * raw;      // byte offset of the scale bytes
+    static constexpr int scales = codes / kGroup;
+    static constexpr int bytes = (scaleAt + scales + 127) / 128 * 128;
+};
+
+// Hot row of slot s of request b: -1 where there is none.  A row past the
+// buffer is none either, and told in the tail-slot word.
+__device__ __forceinline__ int64_t hot_row(int32_t slot, uint64_t b, uint64_t reqStride, uint64_t hotRows,
+                                           uint64_t overflowSlot)
+{
+    if (slot < 0) return -1;
+    const uint64_t row = b * reqStride + static_cast<uint32_t>(slot);
+    if (row >= hotRows) {
+        if (overflowSlot != 0) {
+            atomicCAS(reinterpret_cast<unsigned long long *>(overflowSlot), 0ull, KVX_OVERFLOW_ROW);
+        }
+        return -1;
+    }
+    return static_cast<int64_t>(row);
+}
+
+struct RowCopyArgs {
+    uint64_t rows16;        // the 16-bit (or, reading, 32-bit) rows
+    uint64_t rowStride;     // bytes between them
+    uint64_t hot;
+    uint64_t hotRows;
+    uint64_t slots;         // 0: row i is hot row i
+    uint64_t reqStride;
+    uint64_t rows;          // num_reqs * rows_per_req
+    uint32_t perReq;
+    uint64_t overflowSlot;
+};
+
+hipError_t launch_quantize_rows(const RowCopyArgs &a, uint32_t dtype, uint32_t quant, hipStream_t stream);
+hipError_t launch_dequantize_rows(const RowCopyArgs &a, uint32_t dtype, uint32_t quant, uint32_t outDtype,
+                                  hipStream_t stream);
+
+struct AttnArgs {
+    uint64_t q, qStrideB, qStrideT, qStrideH;   // bytes
+    uint64_t hot, hotRows, reqStride;
+    uint64_t slots, draftSlots, treeMask;
+    uint64_t out, lse;
+    uint32_t reqs, draft, heads, topK;
+    float scaleLog2;        // softmax_scale * log2(e): scores are held in powers of two
+    uint64_t overflowSlot;
+};
+
+hipError_t launch_tree_attention(const AttnArgs &a, uint32_t dtype, uint32_t quant, hipStream_t stream);
+
+}  // namespace kvx

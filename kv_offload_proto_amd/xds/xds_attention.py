@@ -1,0 +1,210 @@
+"""Operators on the cache rows: rows in 8 bits, and attention over the hot buffer.
+
+A row holds ``kv_lora_rank`` latent values, which every query head uses as keys
+and as values, and ``qk_rope`` rotary ones, used as keys only.  The pool, the
+imports and the exports move rows of any ``row_bytes``; these calls read and
+write what is in them, on the slots that ``XdsOffloadCoordinator`` hands out
+(hot row = request * req_stride_rows + slot, -1 = none).  A decode step of one
+layer with 8-bit rows:
+
+    fmt = row_format(torch.bfloat16, quant="row")           # pool made with row_bytes=fmt.row_bytes
+    quantize_rows(fmt, new_rows, hot, new_slots, stride)    # the drafted tokens' own rows
+    coord.sieve_update(layer, topk)
+    pool.batch_read_fused(layer, topk, ...)                 # misses, 640 bytes a row
+    out, lse = tree_attention(fmt, q, hot, coord.top_k_device_slots, scale, stride,
+                              draft_slots=new_slots, tree_mask=mask)
+
+Everything is asynchronous on torch's current stream unless a stream is given,
+and can be recorded into a graph.  The reference has no counterpart: it moves
+rows as bytes.
+"""
+from functools import lru_cache
+from typing import Optional, Tuple
+
+import torch
+
+from ..kvops_ext import _kvops
+from .xds_offload import _stream_handle
+
+_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_QUANTS = {"none": 0, "latent": 1, "row": 2}
+
+
+class RowFormat:
+    """What a cache row holds and where.
+
+    ``quant``: ``"none"`` (every value in 16 bits), ``"latent"`` (the latent
+    values in 8 bits, the rotary ones in 16) or ``"row"`` (all in 8 bits).
+    8-bit values are e4m3 codes with one power-of-two scale for 32 of them,
+    the smallest one under which none exceeds the largest code (448).
+    ``dtype`` is the 16-bit type of the values on the other side.
+    """
+
+    __slots__ = ("dtype", "kv_lora_rank", "qk_rope", "quant", "dim", "row_bytes", "code")
+
+    def __init__(self, dtype=torch.bfloat16, kv_lora_rank: int = 512, qk_rope: int = 64, quant: str = "none"):
+        if dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError("dtype must be bfloat16 or float16, got {}".format(dtype))
+        if (kv_lora_rank, qk_rope) != (512, 64):
+            raise ValueError("rows of kv_lora_rank 512 and qk_rope 64 are supported, got {} and {}".format(
+                kv_lora_rank, qk_rope))
+        if quant not in _QUANTS:
+            raise ValueError("quant must be 'none', 'latent' or 'row', got {!r}".format(quant))
+        self.dtype, self.kv_lora_rank, self.qk_rope, self.quant = dtype, kv_lora_rank, qk_rope, quant
+        self.dim = kv_lora_rank + qk_rope
+        codes = {"none": 0, "latent": kv_lora_rank, "row": self.dim}[quant]
+        self.row_bytes = -(-(codes + 2 * (self.dim - codes) + codes // 32) // 128) * 128
+        self.code = (kv_lora_rank, qk_rope, _DTYPES[dtype], _QUANTS[quant])
+
+    def __repr__(self):
+        return "RowFormat({}, kv_lora_rank={}, qk_rope={}, quant={!r}: {} bytes)".format(
+            self.dtype, self.kv_lora_rank, self.qk_rope, self.quant, self.row_bytes)
+
+
+@lru_cache(maxsize=None)
+def row_format(dtype=torch.bfloat16, kv_lora_rank: int = 512, qk_rope: int = 64, quant: str = "none") -> RowFormat:
+    """The one ``RowFormat`` of these arguments."""
+    return RowFormat(dtype, kv_lora_rank, qk_rope, quant)
+
+
+def _hot(fmt: RowFormat, hot: torch.Tensor) -> int:
+    """Rows of the hot buffer: a contiguous tensor, of any type, whose last
+    dimension is one row of bytes or which holds a whole number of rows."""
+    if not hot.is_cuda:
+        raise ValueError("hot must be on the GPU")
+    if not hot.is_contiguous():
+        raise ValueError("hot must be contiguous")
+    nbytes = hot.numel() * hot.element_size()
+    if nbytes % fmt.row_bytes:
+        raise ValueError("hot holds {} bytes, no multiple of the row's {}".format(nbytes, fmt.row_bytes))
+    return nbytes // fmt.row_bytes
+
+
+def _ints(x: torch.Tensor, name: str, shape, dtype, device) -> int:
+    if x.dtype is not dtype or x.shape != shape or not x.is_contiguous() or x.device != device:
+        raise ValueError("{} must be a contiguous {} tensor of shape {} on {}, got {} of {} on {}".format(
+            name, dtype, tuple(shape), device, x.dtype, tuple(x.shape), x.device))
+    return x.data_ptr()
+
+
+def _slots(slots: Optional[torch.Tensor], rows: int, device) -> Tuple[int, int, int]:
+    """(address, requests, rows of each) of int32 slots [requests, rows]."""
+    if slots is None:
+        return 0, 1, rows
+    if slots.dim() != 2 or slots.numel() != rows:
+        raise ValueError("slots must be [requests, rows of each] with one slot for each of the {} rows, got {}".format(
+            rows, tuple(slots.shape)))
+    return _ints(slots, "slots", slots.shape, torch.int32, device), slots.shape[0], slots.shape[1]
+
+
+def _stride(req_stride_rows: int) -> int:
+    if req_stride_rows < 0:
+        raise ValueError("req_stride_rows must not be negative")
+    return req_stride_rows
+
+
+def _needs_codes(fmt: RowFormat) -> None:
+    if fmt.quant == "none":
+        raise ValueError("rows of format {!r} hold no codes".format(fmt))
+
+
+def quantize_rows(fmt: RowFormat, rows: torch.Tensor, hot: torch.Tensor, slots: Optional[torch.Tensor] = None,
+                  req_stride_rows: int = 0, stream=None) -> None:
+    """Write 16-bit rows [..., dim] (``fmt.dtype``, contiguous but for a stride
+    of the next-to-last dimension) into hot rows of ``fmt``.  Row i goes to the
+    i-th of ``slots`` (int32 [requests, rows of each], negative: left out), or
+    without slots to hot row i.  No two rows may name the same slot."""
+    _needs_codes(fmt)
+    if rows.dtype is not fmt.dtype or rows.shape[-1] != fmt.dim or not rows.is_cuda:
+        raise ValueError("rows must be {} [..., {}] on the GPU, got {} {}".format(
+            fmt.dtype, fmt.dim, rows.dtype, tuple(rows.shape)))
+    if rows.dim() != 2:
+        rows = rows.reshape(-1, fmt.dim)
+    if rows.stride(1) != 1 or rows.stride(0) % 8:
+        rows = rows.contiguous()
+    n, hot_rows = rows.shape[0], _hot(fmt, hot)
+    at, reqs, each = _slots(slots, n, rows.device)
+    if slots is None and n > hot_rows:
+        raise ValueError("{} rows and no slots, but hot holds {}".format(n, hot_rows))
+    _kvops.quantize_rows(rows.data_ptr(), rows.stride(0) * 2, hot.data_ptr(), hot_rows, at, reqs, each,
+                         _stride(req_stride_rows), *fmt.code, _stream_handle(stream))
+
+
+def dequantize_rows(fmt: RowFormat, hot: torch.Tensor, slots: Optional[torch.Tensor] = None,
+                    req_stride_rows: int = 0, out: Optional[torch.Tensor] = None, dtype=None,
+                    stream=None) -> torch.Tensor:
+    """The values of the hot rows that ``slots`` (int32 [requests, rows of
+    each]) name, as [requests * rows, dim] of ``dtype`` (default ``fmt.dtype``;
+    any 16-bit float or float32); zeros where a slot is negative.  Without
+    slots: of every hot row (as many as ``out`` has, where it is given)."""
+    _needs_codes(fmt)
+    hot_rows = _hot(fmt, hot)
+    if out is None:
+        n = hot_rows if slots is None else slots.numel()
+        out = torch.empty((n, fmt.dim), dtype=dtype or fmt.dtype, device=hot.device)
+    elif (out.dtype not in _DTYPES or (dtype is not None and out.dtype is not dtype) or out.shape[-1] != fmt.dim or
+          not out.is_contiguous() or out.device != hot.device):
+        raise ValueError("out must be contiguous, of the dtype asked for, [rows, {}] on {}, got {} {} on {}".format(
+            fmt.dim, hot.device, out.dtype, tuple(out.shape), out.device))
+    n = out.numel() // fmt.dim
+    at, reqs, each = _slots(slots, n, hot.device)
+    if slots is None and n > hot_rows:
+        raise ValueError("{} rows and no slots, but hot holds {}".format(n, hot_rows))
+    _kvops.dequantize_rows(hot.data_ptr(), hot_rows, at, reqs, each, _stride(req_stride_rows), out.data_ptr(),
+                           *fmt.code, _DTYPES[out.dtype], _stream_handle(stream))
+    return out
+
+
+def tree_attention(fmt: RowFormat, q: torch.Tensor, hot: torch.Tensor, slots: torch.Tensor, softmax_scale: float,
+                   req_stride_rows: int = 0, draft_slots: Optional[torch.Tensor] = None,
+                   tree_mask: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                   lse: Optional[torch.Tensor] = None, stream=None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Attention of each request's tokens over its selected rows of the hot
+    buffer, and over the tokens' own.
+
+    ``q`` [requests, tokens, heads, dim] of ``fmt.dtype`` (strided; the last
+    dimension contiguous): the queries of the drafted tokens, one where
+    nothing is drafted.  Every token sees the rows of ``slots`` (int32
+    [requests, topK], ``coord.top_k_device_slots``; -1 = none).  Where
+    ``draft_slots`` (int32 [requests, tokens]) is given, token t also sees the
+    row of token j if bit j of ``tree_mask[request, t]`` is set (int64
+    [requests, tokens]; default: j <= t).  At most 64 tokens.
+
+    Returns ``out`` [requests, tokens, heads, kv_lora_rank] of ``fmt.dtype``,
+    the weighted latent values, and ``lse`` float32 [requests, tokens, heads],
+    the logarithm of the sum of exp(softmax_scale * q.k); 0 and -inf where a
+    query sees no row.  Both can be given (contiguous).
+    """
+    if q.dim() != 4 or q.dtype is not fmt.dtype or q.shape[3] != fmt.dim or not q.is_cuda:
+        raise ValueError("q must be {} [requests, tokens, heads, {}] on the GPU, got {} {}".format(
+            fmt.dtype, fmt.dim, q.dtype, tuple(q.shape)))
+    reqs, tokens, heads, _ = q.shape
+    sb, st, sh, sd = q.stride()
+    if sd != 1 or (sb | st | sh) % 8 or min(sb, st, sh) < 0:
+        raise ValueError("q's last dimension must be contiguous and its other strides multiples of 8, got {}".format(
+            q.stride()))
+    device = q.device
+    hot_rows = _hot(fmt, hot)
+    if slots.dim() != 2 or slots.shape[0] < reqs:
+        raise ValueError("slots must be [requests, topK] with a row for each of the {} requests, got {}".format(
+            reqs, tuple(slots.shape)))
+    at = _ints(slots, "slots", slots.shape, torch.int32, device)
+    d_at = m_at = 0
+    if draft_slots is not None:
+        d_at = _ints(draft_slots, "draft_slots", (reqs, tokens), torch.int32, device)
+        if tree_mask is not None:
+            m_at = _ints(tree_mask, "tree_mask", (reqs, tokens), torch.int64, device)
+    elif tree_mask is not None:
+        raise ValueError("tree_mask needs draft_slots")
+    if out is None:
+        out = torch.empty((reqs, tokens, heads, fmt.kv_lora_rank), dtype=fmt.dtype, device=device)
+    else:
+        _ints(out, "out", (reqs, tokens, heads, fmt.kv_lora_rank), fmt.dtype, device)
+    if lse is None:
+        lse = torch.empty((reqs, tokens, heads), dtype=torch.float32, device=device)
+    else:
+        _ints(lse, "lse", (reqs, tokens, heads), torch.float32, device)
+    _kvops.tree_attention(q.data_ptr(), sb * 2, st * 2, sh * 2, hot.data_ptr(), hot_rows, at, d_at, m_at,
+                          out.data_ptr(), lse.data_ptr(), reqs, tokens, heads, slots.shape[1],
+                          _stride(req_stride_rows), softmax_scale, *fmt.code, _stream_handle(stream))
+    return out, lse

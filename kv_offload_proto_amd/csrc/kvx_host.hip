@@ -13,6 +13,7 @@
 #include <cerrno>
 #include <cctype>
 #include <chrono>
+#include <cmath>
 #include <cstdio>
 #include <cstring>
 #include <fstream>
@@ -50,6 +51,8 @@ struct StreamScratch {
     uint64_t auxWords = 0;
     uint32_t *tbl = nullptr;        // its table rebuild: per-row cells, counts, new keys
     uint64_t tblWords = 0;
+    float *attn = nullptr;          // attention split over workgroups: their outputs
+    uint64_t attnFloats = 0;
 };
 
 // Scratch of kvx_import_all_noalloc: a fixed array in the library's code
@@ -201,7 +204,7 @@ void CheckStatusBlock(uint64_t status, uint32_t firstNode, uint32_t nodes, uint3
 
 // Scratch needs of one launch (entries of each buffer; 0 = not used).
 struct ScratchNeed {
-    uint64_t win = 0, shadow = 0, aux = 0, tbl = 0;
+    uint64_t win = 0, shadow = 0, aux = 0, tbl = 0, attn = 0;
 };
 
 bool Capturing(hipStream_t s)
@@ -235,7 +238,7 @@ StreamScratch &ScratchFor(uint64_t stream, const ScratchNeed &need, const char *
     }
     const bool create = sc == nullptr;
     const bool grow = create || sc->rows.winEntries < need.win || sc->shadowCells < need.shadow ||
-                      sc->auxWords < need.aux || sc->tblWords < need.tbl;
+                      sc->auxWords < need.aux || sc->tblWords < need.tbl || sc->attnFloats < need.attn;
     if (!grow) return *sc;
     hipStream_t st = AsStream(stream);
     if (Capturing(st)) {
@@ -281,6 +284,12 @@ StreamScratch &ScratchFor(uint64_t stream, const ScratchNeed &need, const char *
         if (sc->tbl != nullptr) g.retired.push_back(sc->tbl);
         sc->tbl = static_cast<uint32_t *>(p);
         sc->tblWords = need.tbl;
+    }
+    if (sc->attnFloats < need.attn) {
+        void *p = ScratchAlloc(need.attn * sizeof(float), st, "attention scratch");
+        if (sc->attn != nullptr) g.retired.push_back(sc->attn);
+        sc->attn = static_cast<float *>(p);
+        sc->attnFloats = need.attn;
     }
     return *sc;
 }
@@ -640,7 +649,8 @@ int kvx_scratch_bytes(uint64_t stream, uint64_t *out_bytes)
         for (const StreamScratch *s : g.scratch) {
             if (s->stream != stream) continue;
             b = kvx::kControlWords * sizeof(uint32_t) + s->rows.winEntries * sizeof(unsigned long long) +
-                s->shadowCells * sizeof(int32_t) + s->auxWords * sizeof(uint32_t) + s->tblWords * sizeof(uint32_t);
+                s->shadowCells * sizeof(int32_t) + s->auxWords * sizeof(uint32_t) + s->tblWords * sizeof(uint32_t) +
+                s->attnFloats * sizeof(float);
         }
         *out_bytes = b;
     });
@@ -1132,6 +1142,7 @@ int kvx_close(void)
                 if (s->shadow != nullptr) (void)hipFree(s->shadow);
                 if (s->aux != nullptr) (void)hipFree(s->aux);
                 if (s->tbl != nullptr) (void)hipFree(s->tbl);
+                if (s->attn != nullptr) (void)hipFree(s->attn);
                 delete s;
             }
             g.scratch.clear();
@@ -1226,12 +1237,23 @@ int kvx_tree_attention(uint64_t q, uint64_t q_stride_b, uint64_t q_stride_t, uin
         a.draft = draft;
         a.heads = heads;
         a.topK = top_k;
-        a.scaleLog2 = softmax_scale * 1.4426950408889634f;
+        // a scale of 0 weighs every key alike, as the smallest one does
+        a.scaleLog2 = std::max(std::fabs(softmax_scale) * 1.4426950408889634f, 1e-30f);
+        a.negate = softmax_scale < 0.0f ? 1u : 0u;
         a.overflowSlot = reinterpret_cast<uint64_t>(g.overflow);
         if (static_cast<uint64_t>(num_reqs) * draft * heads >= 1ull << 31) {
             throw Error("tree_attention: num_reqs * draft * heads must be below 2^31");
         }
-        hipCheck(kvx::launch_tree_attention(a, dtype, quant, AsStream(stream)), "tree_attention launch");
+        const kvx::AttnPlan p = kvx::plan_tree_attention(num_reqs, draft, heads, top_k, draft_slots != 0);
+        float *scratch = nullptr;
+        std::unique_lock<std::mutex> lk(g_scratchMu, std::defer_lock);
+        if (p.floats != 0) {
+            ScratchNeed need;
+            need.attn = p.floats;
+            lk.lock();
+            scratch = ScratchFor(stream, need, "tree_attention").attn;
+        }
+        hipCheck(kvx::launch_tree_attention(a, p, scratch, dtype, quant, AsStream(stream)), "tree_attention launch");
     });
 }
 

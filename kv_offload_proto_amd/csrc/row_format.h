@@ -62,10 +62,24 @@ struct AttnArgs {
     uint64_t slots, draftSlots, treeMask;
     uint64_t out, lse;
     uint32_t reqs, draft, heads, topK;
-    float scaleLog2;        // softmax_scale * log2(e): scores are held in powers of two
+    float scaleLog2;        // |softmax_scale| * log2(e), above 0: scores are held in powers of two
+    uint32_t negate;        // softmax_scale is negative
     uint64_t overflowSlot;
+    // set by the launch
+    uint32_t queryTiles, splits;
+    float *part;            // [reqs][splits][queries][512], scaled to the split's own maximum
+    float2 *partStat;       // [reqs][splits][queries]: maximum (power of two), sum
 };
 
-hipError_t launch_tree_attention(const AttnArgs &a, uint32_t dtype, uint32_t quant, hipStream_t stream);
+// How a call is cut up.
+struct AttnPlan {
+    uint32_t rows;          // queries a workgroup: 16, 32, 64 or 128
+    uint32_t queryTiles;    // ... and how many of these a request has
+    uint32_t splits;        // workgroups that share a query's keys
+    uint64_t floats;        // scratch for their outputs
+};
+AttnPlan plan_tree_attention(uint32_t reqs, uint32_t draft, uint32_t heads, uint32_t topK, bool drafted);
+hipError_t launch_tree_attention(AttnArgs a, const AttnPlan &p, float *scratch, uint32_t dtype, uint32_t quant,
+                                 hipStream_t stream);
 
 }  // namespace kvx

@@ -26,10 +26,12 @@ constexpr int kPanels = kDim / 64;        // a row in LDS: 9 panels of 64 values
 constexpr int kPanelBytes = kTile * 128;
 constexpr int kTileBytes = kPanels * kPanelBytes;
 constexpr int kChunk = 64;                // tiles whose rows are looked up at a time
+constexpr int kAhead = 2;                 // panels whose operands are read ahead
 constexpr float kRise = 8.0f;             // a maximum may rise by 2^8 before the output is scaled down again
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -271,8 +273,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
             const uint32_t k = c0 * kTile + i;
             int32_t slot = -1;
             if (i < chunk * kTile && k < keys) {
-                slot = k < a.topK ? reinterpret_cast<const int32_t *>(a.slots)[static_cast<uint64_t>(req) * a.topK + k]
-                                  : reinterpret_cast<const int32_t *>(a.draftSlots)[static_cast<uint64_t>(req) * a.draft + k - a.topK];
+                slot = k < a.topK ? reinterpret_cast<const KVX_GLB int32_t *>(a.slots)[static_cast<uint64_t>(req) * a.topK + k]
+                                  : reinterpret_cast<const KVX_GLB int32_t *>(a.draftSlots)[static_cast<uint64_t>(req) * a.draft + k - a.topK];
             }
             rowOf[i] = hot_row(slot, req, a.reqStride, a.hotRows, a.overflowSlot) < 0 ? -1 : slot;
         }
@@ -290,16 +292,27 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
             if (live == 0 && !(drafted && WR > 1)) return;
             const KVX_LDS uint8_t *tile = (KVX_LDS uint8_t *)(uintptr_t)(ldsGroup + buffer * kTileBytes);
 
+            // the operands of the next panels are on their way while one panel's are multiplied
             f32x4 s[2][RW] = {};
+            u32x4 key[kAhead + 1][4];
+            auto readKeys = [&](int p) {
 #pragma unroll
-            for (int st = 0; st < kDim / 32; ++st) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const u32x4 k = *reinterpret_cast<const KVX_LDS u32x4 *>(tile + atKey[st & 1] + (st >> 1) * kPanelBytes + h * 2048);
-#pragma unroll
-                    for (int w = 0; w < RW; ++w) s[h][w] = E::mfma(k, q[w][st], s[h][w]);
+                for (int i = 0; i < 4; ++i) {
+                    key[p % (kAhead + 1)][i] = *reinterpret_cast<const KVX_LDS u32x4 *>(tile + atKey[i >> 1] + p * kPanelBytes + (i & 1) * 2048);
                 }
-                if (st % 3 == 2) __builtin_amdgcn_sched_barrier(0);
+            };
+#pragma unroll
+            for (int p = 0; p < kAhead; ++p) readKeys(p);
+#pragma unroll
+            for (int p = 0; p < kPanels; ++p) {
+                if (p + kAhead < kPanels) readKeys(p + kAhead);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+#pragma unroll
+                    for (int w = 0; w < RW; ++w) s[i & 1][w] = E::mfma(key[p % (kAhead + 1)][i], q[w][p * 2 + (i >> 1)], s[i & 1][w]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
             }
             if (live != ~0u || drafted) {
                 const uint32_t selected = k0 >= a.topK ? 0u : (a.topK - k0 >= 32u ? ~0u : (1u << (a.topK - k0)) - 1u);
@@ -342,18 +355,6 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
                     }
                 }
             }
-            u32x4 weight[RW];
-#pragma unroll
-            for (int w = 0; w < RW; ++w) {
-                const float base = top[w] == -INFINITY ? 0.0f : top[w];
-                float p[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j >> 2][w][j & 3], a.scaleLog2, -base));
-                    sum[w] += p[j];
-                }
-                weight[w] = u32x4{pack2<T>(p[0], p[1]), pack2<T>(p[2], p[3]), pack2<T>(p[4], p[5]), pack2<T>(p[6], p[7])};
-            }
             // A drafted row that holds a NaN or an infinity must not reach the
             // queries that do not see it, whose weight 0 would turn it into a NaN;
             // those that see it have a score that is one already.
@@ -371,15 +372,40 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
                 }
                 if (WR > 1) meet();
             }
+            u32x4 value[kAhead + 1][4];
+            auto readValues = [&](int p) {
 #pragma unroll
-            for (int d = 0; d < kLatent / 16; ++d) {
-                KVX_LDS s16x4 *at = (KVX_LDS s16x4 *)(tile + atValue[d & 3] + (d >> 2) * kPanelBytes);
-                const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at);
-                const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at + 2048 / 8);
-                const u32x4 v = __builtin_bit_cast(u32x4, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+                for (int i = 0; i < 4; ++i) {
+                    KVX_LDS s16x4 *at = (KVX_LDS s16x4 *)(tile + atValue[i] + p * kPanelBytes);
+                    const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at);
+                    const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at + 2048 / 8);
+                    value[p % (kAhead + 1)][i] = __builtin_bit_cast(u32x4, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+                }
+            };
 #pragma unroll
-                for (int w = 0; w < RW; ++w) o[d][w] = E::mfma(v, weight[w], o[d][w]);
-                if (d % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+            for (int p = 0; p < kAhead; ++p) readValues(p);
+            u32x4 weight[RW];
+#pragma unroll
+            for (int w = 0; w < RW; ++w) {
+                const float base = top[w] == -INFINITY ? 0.0f : top[w];
+                float p[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j >> 2][w][j & 3], a.scaleLog2, -base));
+                    sum[w] += p[j];
+                }
+                weight[w] = u32x4{pack2<T>(p[0], p[1]), pack2<T>(p[2], p[3]), pack2<T>(p[4], p[5]), pack2<T>(p[6], p[7])};
+            }
+#pragma unroll
+            for (int p = 0; p < kLatent / 64; ++p) {
+                if (p + kAhead < kLatent / 64) readValues(p + kAhead);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+#pragma unroll
+                    for (int w = 0; w < RW; ++w) o[p * 4 + i][w] = E::mfma(value[p % (kAhead + 1)][i], weight[w], o[p * 4 + i][w]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
             }
         };
 
@@ -466,14 +492,14 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
                 stat[wr][w * 16 + col][1] = sum[w];
             }
         }
-        float *join = reinterpret_cast<float *>(tiles);
+        KVX_LDS float *join = (KVX_LDS float *)tiles;
 #pragma unroll
         for (int round = 0; round < RW; ++round) {
 #pragma unroll
             for (int d = 0; d < kJoinCols / 16; ++d) {
 #pragma unroll
                 for (int w = 0; w < RW; ++w) {
-                    *reinterpret_cast<f32x4 *>(join + (wave * kRows + w * 16 + col) * kJoinStride + d * 16 + grp * 4) =
+                    *reinterpret_cast<KVX_LDS f32x4 *>(join + (wave * kRows + w * 16 + col) * kJoinStride + d * 16 + grp * 4) =
                         o[round * (kJoinCols / 16) + d][w];
                 }
             }
@@ -482,17 +508,17 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
                 const uint32_t c = i % (kJoinCols / 4), r = i / (kJoinCols / 4);
                 f32x4 x = {};
 #pragma unroll
-                for (int g = 0; g < WK; ++g) x += *reinterpret_cast<const f32x4 *>(join + (g * WR * kRows + r) * kJoinStride + c * 4);
+                for (int g = 0; g < WK; ++g) x += *reinterpret_cast<const KVX_LDS f32x4 *>(join + (g * WR * kRows + r) * kJoinStride + c * 4);
                 const uint32_t index = qt * WR * kRows + r;
                 const float all = stat[r / kRows][r % kRows][1];
                 if (index < queries) {
                     if (a.splits == 1) {
                         const float inv = all == 0.0f ? 0.0f : 1.0f / all;
-                        T *out = reinterpret_cast<T *>(a.out) + (row0 + index) * kLatent + round * kJoinCols + c * 4;
-                        *reinterpret_cast<u32x2 *>(out) = u32x2{pack2<T>(x[0] * inv, x[1] * inv), pack2<T>(x[2] * inv, x[3] * inv)};
+                        KVX_GLB T *out = reinterpret_cast<KVX_GLB T *>(a.out) + (row0 + index) * kLatent + round * kJoinCols + c * 4;
+                        *reinterpret_cast<KVX_GLB u32x2 *>(out) = u32x2{pack2<T>(x[0] * inv, x[1] * inv), pack2<T>(x[2] * inv, x[3] * inv)};
                     } else {
-                        float *out = a.part + ((static_cast<uint64_t>(req) * a.splits + split) * queries + index) * kLatent + round * kJoinCols + c * 4;
-                        *reinterpret_cast<f32x4 *>(out) = x;
+                        KVX_GLB float *out = reinterpret_cast<KVX_GLB float *>(a.part) + ((static_cast<uint64_t>(req) * a.splits + split) * queries + index) * kLatent + round * kJoinCols + c * 4;
+                        *reinterpret_cast<KVX_GLB f32x4 *>(out) = x;
                     }
                 }
             }
@@ -504,19 +530,19 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
             if (query[w] >= queries) continue;
             if (a.splits == 1) {
                 const float inv = sum[w] == 0.0f ? 0.0f : 1.0f / sum[w];
-                T *out = reinterpret_cast<T *>(a.out) + (row0 + query[w]) * kLatent + grp * 4;
+                KVX_GLB T *out = reinterpret_cast<KVX_GLB T *>(a.out) + (row0 + query[w]) * kLatent + grp * 4;
 #pragma unroll
                 for (int d = 0; d < kLatent / 16; ++d) {
                     keep_in_acc(o[d][w]);
-                    *reinterpret_cast<u32x2 *>(out + d * 16) =
+                    *reinterpret_cast<KVX_GLB u32x2 *>(out + d * 16) =
                         u32x2{pack2<T>(o[d][w][0] * inv, o[d][w][1] * inv), pack2<T>(o[d][w][2] * inv, o[d][w][3] * inv)};
                 }
             } else {
-                float *out = a.part + ((static_cast<uint64_t>(req) * a.splits + split) * queries + query[w]) * kLatent + grp * 4;
+                KVX_GLB float *out = reinterpret_cast<KVX_GLB float *>(a.part) + ((static_cast<uint64_t>(req) * a.splits + split) * queries + query[w]) * kLatent + grp * 4;
 #pragma unroll
                 for (int d = 0; d < kLatent / 16; ++d) {
                     keep_in_acc(o[d][w]);
-                    *reinterpret_cast<f32x4 *>(out + d * 16) = o[d][w];
+                    *reinterpret_cast<KVX_GLB f32x4 *>(out + d * 16) = o[d][w];
                 }
             }
         }
@@ -527,11 +553,11 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
             if (query[w] >= queries) continue;
             if (a.splits == 1) {
                 if (a.lse != 0) {
-                    reinterpret_cast<float *>(a.lse)[row0 + query[w]] =
+                    reinterpret_cast<KVX_GLB float *>(a.lse)[row0 + query[w]] =
                         sum[w] == 0.0f ? -INFINITY : (top[w] + __builtin_amdgcn_logf(sum[w])) * 0.6931471805599453f;
                 }
             } else {
-                a.partStat[(static_cast<uint64_t>(req) * a.splits + split) * queries + query[w]] = float2{top[w], sum[w]};
+                reinterpret_cast<KVX_GLB f32x2 *>(a.partStat)[(static_cast<uint64_t>(req) * a.splits + split) * queries + query[w]] = f32x2{top[w], sum[w]};
             }
         }
     }
@@ -547,25 +573,26 @@ __global__ __launch_bounds__(kThreads) void kvx_tree_attention_join(AttnArgs a)
     if (row >= static_cast<uint64_t>(a.reqs) * queries) return;
     const uint32_t lane = threadIdx.x & 63u;
     const uint64_t first = row / queries * a.splits * queries + row % queries;
+    const KVX_GLB f32x2 *stats = reinterpret_cast<const KVX_GLB f32x2 *>(a.partStat) + first;
     float most = -INFINITY;
-    for (uint32_t s = 0; s < a.splits; ++s) most = fmaxf(most, a.partStat[first + static_cast<uint64_t>(s) * queries].x);
+    for (uint32_t s = 0; s < a.splits; ++s) most = fmaxf(most, stats[static_cast<uint64_t>(s) * queries].x);
     const float base = most == -INFINITY ? 0.0f : most;
     float all = 0.0f;
     f32x4 x = {}, y = {};
     for (uint32_t s = 0; s < a.splits; ++s) {
         const uint64_t at = first + static_cast<uint64_t>(s) * queries;
-        const float2 st = a.partStat[at];
+        const f32x2 st = stats[static_cast<uint64_t>(s) * queries];
         const float keep = __builtin_amdgcn_exp2f(st.x - base);
         all += st.y * keep;
-        const f32x4 *v = reinterpret_cast<const f32x4 *>(a.part + at * kLatent) + lane * 2;
+        const KVX_GLB f32x4 *v = reinterpret_cast<const KVX_GLB f32x4 *>(a.part) + at * (kLatent / 4) + lane * 2;
         x += v[0] * keep;
         y += v[1] * keep;
     }
     const float inv = all == 0.0f ? 0.0f : 1.0f / all;
-    *reinterpret_cast<u32x4 *>(reinterpret_cast<T *>(a.out) + row * kLatent + lane * 8) =
+    *reinterpret_cast<KVX_GLB u32x4 *>(reinterpret_cast<KVX_GLB T *>(a.out) + row * kLatent + lane * 8) =
         u32x4{pack2<T>(x[0] * inv, x[1] * inv), pack2<T>(x[2] * inv, x[3] * inv), pack2<T>(y[0] * inv, y[1] * inv), pack2<T>(y[2] * inv, y[3] * inv)};
     if (lane == 0 && a.lse != 0) {
-        reinterpret_cast<float *>(a.lse)[row] = all == 0.0f ? -INFINITY : (most + __builtin_amdgcn_logf(all)) * 0.6931471805599453f;
+        reinterpret_cast<KVX_GLB float *>(a.lse)[row] = all == 0.0f ? -INFINITY : (most + __builtin_amdgcn_logf(all)) * 0.6931471805599453f;
     }
 }
 
@@ -606,8 +633,8 @@ hipError_t launch_tree_attention(AttnArgs a, const AttnPlan &p, float *scratch, 
 {
     a.queryTiles = p.queryTiles;
     a.splits = p.splits;
-    a.part = scratch;
-    a.partStat = reinterpret_cast<float2 *>(scratch + static_cast<uint64_t>(a.reqs) * p.splits * a.draft * a.heads * kLatent);
+    a.part = reinterpret_cast<uint64_t>(scratch);
+    a.partStat = a.part + static_cast<uint64_t>(a.reqs) * p.splits * a.draft * a.heads * kLatent * sizeof(float);
     if (dtype == KVX_DTYPE_BF16) {
         if (quant == KVX_QUANT_NONE) launch<KVX_DTYPE_BF16, KVX_QUANT_NONE>(a, p, stream);
         else if (quant == KVX_QUANT_LATENT) launch<KVX_DTYPE_BF16, KVX_QUANT_LATENT>(a, p, stream);

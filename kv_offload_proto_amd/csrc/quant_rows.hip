@@ -6,20 +6,46 @@
 // values, so with A = m 2^E, 1 <= m < 2, and 448 = 1.75 * 2^8 the exponent is
 // E - 8, plus one where m > 1.75; and the division is by a power of two.
 //
-// One wave per row.
+// Both kernels are copies that convert on the way and are bound by memory: a
+// lane takes 16 values (32 bytes on one side, 16 on the other), 36 lanes a row,
+// and a workgroup of 192 lanes takes 16 rows, three units a lane, whose loads
+// are all issued before the first value is used.  16 rows rather than more
+// keep several workgroups busy in the calls of one decode step.
 #include "row_format.h"
 
 namespace kvx {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kWavesPerBlock = kThreads / 64;
+constexpr int kThreads = 192;
+constexpr int kRowsPerBlock = 16;
+constexpr int kUnits = kDim / 16;                                        // of a row
+constexpr int kUnitsPerLane = kRowsPerBlock * kUnits / kThreads;
+static_assert(kRowsPerBlock * kUnits == kThreads * kUnitsPerLane, "whole units a lane");
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+#define KVX_GLB __attribute__((address_space(1)))
 
 template <int DTYPE>
-__device__ __forceinline__ float to_float(uint16_t bits)
+__device__ __forceinline__ float to_float(uint32_t bits)
 {
-    if constexpr (DTYPE == KVX_DTYPE_BF16) return __uint_as_float(static_cast<uint32_t>(bits) << 16);
-    return static_cast<float>(__builtin_bit_cast(_Float16, bits));
+    if constexpr (DTYPE == KVX_DTYPE_BF16) return __uint_as_float(bits << 16);
+    return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(bits)));
+}
+
+// Two values rounded to 16 bits, packed.
+template <int DTYPE>
+__device__ __forceinline__ uint32_t pack2(float a, float b)
+{
+    if constexpr (DTYPE == KVX_DTYPE_BF16) {
+        typedef __bf16 T2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, T2{static_cast<__bf16>(a), static_cast<__bf16>(b)});
+    } else {
+        typedef _Float16 T2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, T2{static_cast<_Float16>(a), static_cast<_Float16>(b)});
+    }
 }
 
 // Magnitude bits of a finite value, 0 for an infinity or a NaN: ordered as the values are.
@@ -39,83 +65,164 @@ __device__ __forceinline__ uint32_t scale_byte(uint32_t top)
 // 448 limits what only an infinity exceeds; the conversion would make it a NaN.
 __device__ __forceinline__ float limit(float x) { return x != x ? x : fminf(fmaxf(x, -448.0f), 448.0f); }
 
+__device__ __forceinline__ int64_t row_at(const RowCopyArgs &a, uint64_t row)
+{
+    if (row >= a.rows) return -1;
+    if (a.slots == 0) return static_cast<int64_t>(row);
+    return hot_row(reinterpret_cast<const KVX_GLB int32_t *>(a.slots)[row], static_cast<uint32_t>(row) / a.perReq,
+                   a.reqStride, a.hotRows, a.overflowSlot);
+}
+
 template <int DTYPE, int QUANT>
 __global__ __launch_bounds__(kThreads) void kvx_quantize_rows(RowCopyArgs a)
 {
     using F = RowForm<QUANT>;
-    const uint64_t row = static_cast<uint64_t>(blockIdx.x) * kWavesPerBlock + (threadIdx.x >> 6);
-    const uint32_t lane = threadIdx.x & 63u;
-    if (row >= a.rows) return;
-    int64_t to = static_cast<int64_t>(row);
-    if (a.slots != 0) {
-        to = hot_row(reinterpret_cast<const int32_t *>(a.slots)[row], row / a.perReq, a.reqStride, a.hotRows,
-                     a.overflowSlot);
+    constexpr int kTail = F::bytes - F::scaleAt;                         // scale bytes and zeros
+    __shared__ int64_t to[kRowsPerBlock];
+    __shared__ __align__(16) uint8_t tail[kRowsPerBlock][kTail];
+    const uint64_t row0 = static_cast<uint64_t>(blockIdx.x) * kRowsPerBlock;
+
+    u32x4 x[kUnitsPerLane][2];
+#pragma unroll
+    for (int i = 0; i < kUnitsPerLane; ++i) {
+        const uint32_t u = threadIdx.x + i * kThreads, r = u / kUnits, c = u % kUnits;
+        const uint64_t row = row0 + r < a.rows ? row0 + r : a.rows - 1;
+        const KVX_GLB u32x4 *from = reinterpret_cast<const KVX_GLB u32x4 *>(a.rows16 + row * a.rowStride + c * 32);
+        x[i][0] = __builtin_nontemporal_load(from);
+        x[i][1] = __builtin_nontemporal_load(from + 1);
     }
-    if (to < 0) return;
-    const uint16_t *src = reinterpret_cast<const uint16_t *>(a.rows16 + row * a.rowStride);
-    uint8_t *dst = reinterpret_cast<uint8_t *>(a.hot) + static_cast<uint64_t>(to) * F::bytes;
-    // a lane takes a pair of values: 16 lanes a group, 4 groups at a time
-    for (int c = 0; c < F::codes; c += 128) {
-        const int at = c + static_cast<int>(lane) * 2;
-        const bool in = at < F::codes;
-        const float x0 = in ? to_float<DTYPE>(src[at]) : 0.0f, x1 = in ? to_float<DTYPE>(src[at + 1]) : 0.0f;
-        uint32_t top = max(finite_bits(x0), finite_bits(x1));
-        for (int d = 1; d < 16; d <<= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), d)));
+    if (threadIdx.x < kRowsPerBlock) to[threadIdx.x] = row_at(a, row0 + threadIdx.x);
+    for (uint32_t z = threadIdx.x; z < kRowsPerBlock * kTail / 4; z += kThreads) reinterpret_cast<uint32_t *>(tail)[z] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kUnitsPerLane; ++i) {
+        const uint32_t u = threadIdx.x + i * kThreads, r = u / kUnits, c = u % kUnits;
+        float v[16];
+        uint32_t top = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const uint32_t w = x[i][j >> 2][j & 3];
+            v[2 * j] = to_float<DTYPE>(w & 0xFFFFu);
+            v[2 * j + 1] = to_float<DTYPE>(w >> 16);
+            top = max(top, max(finite_bits(v[2 * j]), finite_bits(v[2 * j + 1])));
+        }
+        // the other half of the group is the neighbour's (36 units a row: pairs do not part)
+        top = max(top, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(top), 0xB1, 0xF, 0xF, true)));
         const uint32_t byte = scale_byte(top);
         const float inv = __uint_as_float((254u - byte) << 23);
-        const int pair = __builtin_amdgcn_cvt_pk_fp8_f32(limit(x0 * inv), limit(x1 * inv), 0, false);
-        if (in) {
-            *reinterpret_cast<uint16_t *>(dst + at) = static_cast<uint16_t>(pair);
-            if ((lane & 15u) == 0) dst[F::scaleAt + at / kGroup] = static_cast<uint8_t>(byte);
+        u32x4 codes;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            int two = __builtin_amdgcn_cvt_pk_fp8_f32(limit(v[4 * j] * inv), limit(v[4 * j + 1] * inv), 0, false);
+            two = __builtin_amdgcn_cvt_pk_fp8_f32(limit(v[4 * j + 2] * inv), limit(v[4 * j + 3] * inv), two, true);
+            codes[j] = static_cast<uint32_t>(two);
         }
+        const int64_t row = to[r];
+        const uint64_t dst = a.hot + static_cast<uint64_t>(row) * F::bytes;
+        if (row >= 0) {
+            if (F::raw == 0 || c < F::codes / 16) {
+                *reinterpret_cast<KVX_GLB u32x4 *>(dst + c * 16) = codes;
+            } else {
+                KVX_GLB u32x4 *raw = reinterpret_cast<KVX_GLB u32x4 *>(dst + F::codes + (c - F::codes / 16) * 32);
+                raw[0] = x[i][0];
+                raw[1] = x[i][1];
+            }
+        }
+        if ((c & 1u) == 0 && (F::raw == 0 || c < F::codes / 16)) tail[r][c / 2] = static_cast<uint8_t>(byte);
     }
-    for (int r = static_cast<int>(lane); r < F::raw; r += 64) {
-        reinterpret_cast<uint16_t *>(dst + F::codes)[r] = src[F::codes + r];
+    __syncthreads();
+    for (uint32_t z = threadIdx.x; z < kRowsPerBlock * (kTail / 16); z += kThreads) {
+        const uint32_t r = z / (kTail / 16), c = z % (kTail / 16);
+        if (to[r] < 0) continue;
+        *reinterpret_cast<KVX_GLB u32x4 *>(a.hot + static_cast<uint64_t>(to[r]) * F::bytes + F::scaleAt + c * 16) =
+            *reinterpret_cast<const u32x4 *>(&tail[r][c * 16]);
     }
-    for (int z = F::scaleAt + F::scales + static_cast<int>(lane); z < F::bytes; z += 64) dst[z] = 0;
 }
 
 template <int DTYPE, int QUANT, int OUT>
 __global__ __launch_bounds__(kThreads) void kvx_dequantize_rows(RowCopyArgs a)
 {
     using F = RowForm<QUANT>;
-    const uint64_t row = static_cast<uint64_t>(blockIdx.x) * kWavesPerBlock + (threadIdx.x >> 6);
-    if (row >= a.rows) return;
-    int64_t from = static_cast<int64_t>(row);
-    if (a.slots != 0) {
-        from = hot_row(reinterpret_cast<const int32_t *>(a.slots)[row], row / a.perReq, a.reqStride, a.hotRows,
-                       a.overflowSlot);
-    }
-    const uint8_t *src = reinterpret_cast<const uint8_t *>(a.hot) + static_cast<uint64_t>(from) * F::bytes;
-    for (int at = static_cast<int>(threadIdx.x & 63u); at < kDim; at += 64) {
-        float x = 0.0f;
-        if (from >= 0 && at < F::codes) {
-            const uint32_t byte = src[F::scaleAt + at / kGroup];
-            const float scale = __uint_as_float(byte == 0 ? 0x00400000u : byte << 23);
-            x = __builtin_amdgcn_cvt_f32_fp8(static_cast<int>(src[at]), 0) * scale;
-        } else if (from >= 0) {
-            x = to_float<DTYPE>(reinterpret_cast<const uint16_t *>(src + F::codes)[at - F::codes]);
+    constexpr int kTailUnits = (F::scales + 15) / 16;
+    __shared__ int64_t from[kRowsPerBlock];
+    __shared__ __align__(16) uint8_t scales[kRowsPerBlock][kTailUnits * 16];
+    const uint64_t row0 = static_cast<uint64_t>(blockIdx.x) * kRowsPerBlock;
+    if (threadIdx.x < kRowsPerBlock) from[threadIdx.x] = row_at(a, row0 + threadIdx.x);
+    __syncthreads();
+    // 8 values a lane and unit: stores of 16 bytes that follow each other
+    u32x4 x[2 * kUnitsPerLane];
+#pragma unroll
+    for (int i = 0; i < 2 * kUnitsPerLane; ++i) {
+        const uint32_t u = threadIdx.x + i * kThreads, r = u / (2 * kUnits), c = u % (2 * kUnits);
+        x[i] = u32x4{0, 0, 0, 0};
+        if (from[r] >= 0) {
+            const uint64_t src = a.hot + static_cast<uint64_t>(from[r]) * F::bytes;
+            if (F::raw == 0 || c < F::codes / 8) {
+                const u32x2 codes = *reinterpret_cast<const KVX_GLB u32x2 *>(src + c * 8);
+                x[i][0] = codes[0];
+                x[i][1] = codes[1];
+            } else {
+                x[i] = *reinterpret_cast<const KVX_GLB u32x4 *>(src + F::codes + (c - F::codes / 8) * 16);
+            }
         }
-        if constexpr (OUT == KVX_DTYPE_FP32) {
-            reinterpret_cast<float *>(a.rows16)[row * kDim + at] = x;
-        } else if constexpr (OUT == KVX_DTYPE_BF16) {
-            reinterpret_cast<__bf16 *>(a.rows16)[row * kDim + at] = static_cast<__bf16>(x);
+    }
+    // the scale bytes once for the row: 16 bytes a lane, not one byte a unit
+    if (threadIdx.x < kRowsPerBlock * kTailUnits) {
+        const uint32_t r = threadIdx.x / kTailUnits, c = threadIdx.x % kTailUnits;
+        u32x4 z = {};
+        if (from[r] >= 0) {
+            z = *reinterpret_cast<const KVX_GLB u32x4 *>(a.hot + static_cast<uint64_t>(from[r]) * F::bytes + F::scaleAt + c * 16);
+        }
+        *reinterpret_cast<u32x4 *>(&scales[r][c * 16]) = z;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2 * kUnitsPerLane; ++i) {
+        const uint32_t u = threadIdx.x + i * kThreads, r = u / (2 * kUnits), c = u % (2 * kUnits);
+        if (row0 + r >= a.rows) continue;
+        float v[8];
+        if (F::raw == 0 || c < F::codes / 8) {
+            // 2^-127 has no normal form
+            const uint32_t byte = scales[r][c / 4];
+            const float scale = __uint_as_float(byte == 0 ? 0x00400000u : byte << 23);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(x[i][j]), false);
+                const f32x2 hi = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(x[i][j]), true);
+                v[4 * j] = lo[0] * scale;
+                v[4 * j + 1] = lo[1] * scale;
+                v[4 * j + 2] = hi[0] * scale;
+                v[4 * j + 3] = hi[1] * scale;
+            }
         } else {
-            reinterpret_cast<_Float16 *>(a.rows16)[row * kDim + at] = static_cast<_Float16>(x);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                v[2 * j] = to_float<DTYPE>(x[i][j] & 0xFFFFu);
+                v[2 * j + 1] = to_float<DTYPE>(x[i][j] >> 16);
+            }
+        }
+        const uint64_t at = (row0 + r) * kDim + c * 8;
+        if constexpr (OUT == KVX_DTYPE_FP32) {
+            KVX_GLB f32x4 *out = reinterpret_cast<KVX_GLB f32x4 *>(a.rows16 + at * 4);
+            out[0] = f32x4{v[0], v[1], v[2], v[3]};
+            out[1] = f32x4{v[4], v[5], v[6], v[7]};
+        } else {
+            __builtin_nontemporal_store(u32x4{pack2<OUT>(v[0], v[1]), pack2<OUT>(v[2], v[3]), pack2<OUT>(v[4], v[5]), pack2<OUT>(v[6], v[7])},
+                                        reinterpret_cast<KVX_GLB u32x4 *>(a.rows16 + at * 2));
         }
     }
 }
 
+dim3 row_grid(uint64_t rows) { return dim3(static_cast<uint32_t>((rows + kRowsPerBlock - 1) / kRowsPerBlock)); }
+
 template <int DTYPE, int QUANT>
-void dequantize(const RowCopyArgs &a, uint32_t outDtype, dim3 grid, hipStream_t stream)
+void dequantize(const RowCopyArgs &a, uint32_t outDtype, hipStream_t stream)
 {
     auto *kernel = outDtype == KVX_DTYPE_BF16   ? kvx_dequantize_rows<DTYPE, QUANT, KVX_DTYPE_BF16>
                    : outDtype == KVX_DTYPE_FP16 ? kvx_dequantize_rows<DTYPE, QUANT, KVX_DTYPE_FP16>
                                                 : kvx_dequantize_rows<DTYPE, QUANT, KVX_DTYPE_FP32>;
-    hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL(kernel, row_grid(a.rows), dim3(kThreads), 0, stream, a);
 }
-
-dim3 row_grid(uint64_t rows) { return dim3(static_cast<uint32_t>((rows + kWavesPerBlock - 1) / kWavesPerBlock)); }
 
 }  // namespace
 
@@ -134,11 +241,11 @@ hipError_t launch_dequantize_rows(const RowCopyArgs &a, uint32_t dtype, uint32_t
                                   hipStream_t stream)
 {
     if (dtype == KVX_DTYPE_BF16) {
-        if (quant == KVX_QUANT_LATENT) dequantize<KVX_DTYPE_BF16, KVX_QUANT_LATENT>(a, outDtype, row_grid(a.rows), stream);
-        else dequantize<KVX_DTYPE_BF16, KVX_QUANT_ROW>(a, outDtype, row_grid(a.rows), stream);
+        if (quant == KVX_QUANT_LATENT) dequantize<KVX_DTYPE_BF16, KVX_QUANT_LATENT>(a, outDtype, stream);
+        else dequantize<KVX_DTYPE_BF16, KVX_QUANT_ROW>(a, outDtype, stream);
     } else {
-        if (quant == KVX_QUANT_LATENT) dequantize<KVX_DTYPE_FP16, KVX_QUANT_LATENT>(a, outDtype, row_grid(a.rows), stream);
-        else dequantize<KVX_DTYPE_FP16, KVX_QUANT_ROW>(a, outDtype, row_grid(a.rows), stream);
+        if (quant == KVX_QUANT_LATENT) dequantize<KVX_DTYPE_FP16, KVX_QUANT_LATENT>(a, outDtype, stream);
+        else dequantize<KVX_DTYPE_FP16, KVX_QUANT_ROW>(a, outDtype, stream);
     }
     return hipGetLastError();
 }

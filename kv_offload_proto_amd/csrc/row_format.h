@@ -33,7 +33,12 @@ __device__ __forceinline__ int64_t hot_row(int32_t slot, uint64_t b, uint64_t re
     const uint64_t row = b * reqStride + static_cast<uint32_t>(slot);
     if (row >= hotRows) {
         if (overflowSlot != 0) {
-            atomicCAS(reinterpret_cast<unsigned long long *>(overflowSlot), 0ull, KVX_OVERFLOW_ROW);
+            // (the global address space: a flat access would have later LDS reads waited for in full)
+            typedef __attribute__((address_space(1))) unsigned long long Word;
+            unsigned long long none = 0;
+            __hip_atomic_compare_exchange_strong(reinterpret_cast<Word *>(overflowSlot), &none,
+                                                 static_cast<unsigned long long>(KVX_OVERFLOW_ROW), __ATOMIC_RELAXED,
+                                                 __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
         return -1;
     }
@@ -67,8 +72,8 @@ struct AttnArgs {
     uint64_t overflowSlot;
     // set by the launch
     uint32_t queryTiles, splits;
-    float *part;            // [reqs][splits][queries][512], scaled to the split's own maximum
-    float2 *partStat;       // [reqs][splits][queries]: maximum (power of two), sum
+    uint64_t part;          // float [reqs][splits][queries][512], scaled to the split's own maximum
+    uint64_t partStat;      // float2 [reqs][splits][queries]: maximum (power of two), sum
 };
 
 // How a call is cut up.

@@ -141,7 +141,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
 
     __shared__ __align__(128) uint8_t tiles[kTilesBytes > kJoinBytes ? kTilesBytes : kJoinBytes];
     __shared__ int32_t rowOf[kChunk * kTile];        // hot row within the request of each key, -1: none
-    __shared__ float stat[4][kRows][2];
+    __shared__ float stat[4][kRows][2], weigh[4][kRows];
 
     const uint32_t lane = threadIdx.x & 63u;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -156,10 +156,35 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
     const uint32_t qt = item % a.queryTiles, split = item / a.queryTiles % a.splits;
     const uint32_t req = item / a.queryTiles / a.splits;
 
+    const uint32_t keys = a.topK + (a.draftSlots != 0 ? a.draft : 0u);
+    const uint32_t allTiles = (keys + kTile - 1) / kTile;
+    const uint32_t tile0 = static_cast<uint32_t>(static_cast<uint64_t>(allTiles) * split / a.splits);
+    const uint32_t tile1 = static_cast<uint32_t>(static_cast<uint64_t>(allTiles) * (split + 1) / a.splits);
+    // slots of the chunk from tile c0 on, kThreads apart (-1 past the range)
+    constexpr int kSlots = kChunk * kTile / kThreads;
+    auto readSlots = [&](uint32_t c0, int32_t (&slot)[kSlots]) {
+#pragma unroll
+        for (int n = 0; n < kSlots; ++n) {
+            const uint32_t k = c0 * kTile + n * kThreads + threadIdx.x;
+            slot[n] = -1;
+            if (k < min(keys, tile1 * kTile)) {
+                slot[n] = k < a.topK ? reinterpret_cast<const KVX_GLB int32_t *>(a.slots)[static_cast<uint64_t>(req) * a.topK + k]
+                                     : reinterpret_cast<const KVX_GLB int32_t *>(a.draftSlots)[static_cast<uint64_t>(req) * a.draft + k - a.topK];
+            }
+        }
+    };
+    auto lookUp = [&](const int32_t (&slot)[kSlots]) {
+#pragma unroll
+        for (int n = 0; n < kSlots; ++n) {
+            rowOf[n * kThreads + threadIdx.x] = hot_row(slot[n], req, a.reqStride, a.hotRows, a.overflowSlot) < 0 ? -1 : slot[n];
+        }
+    };
+    int32_t firstSlots[kSlots];
+    readSlots(tile0, firstSlots);                    // (before the queries: the rows' addresses wait for them)
+
     uint32_t query[RW];
     u32x4 q[RW][kDim / 32];
     uint64_t sees[RW];                               // drafted tokens that the query sees
-    const uint32_t flip = a.negate ? 0x80008000u : 0u;
 #pragma unroll
     for (int w = 0; w < RW; ++w) {
         query[w] = (qt * WR + wr) * kRows + w * 16 + col;
@@ -167,9 +192,16 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
         const uint32_t node = real / a.heads, head = real % a.heads;
         const uint64_t at = a.q + req * a.qStrideB + node * a.qStrideT + head * a.qStrideH + grp * 16;
 #pragma unroll
-        for (int s = 0; s < kDim / 32; ++s) q[w][s] = *reinterpret_cast<const KVX_GLB u32x4 *>(at + s * 64) ^ flip;
+        for (int s = 0; s < kDim / 32; ++s) q[w][s] = *reinterpret_cast<const KVX_GLB u32x4 *>(at + s * 64);
         sees[w] = a.treeMask != 0 ? reinterpret_cast<const KVX_GLB uint64_t *>(a.treeMask)[req * a.draft + node]
                                   : ~0ull >> (63u - node);
+    }
+    lookUp(firstSlots);
+    const uint32_t flip = a.negate ? 0x80008000u : 0u;               // a negative scale: negative queries
+#pragma unroll
+    for (int w = 0; w < RW; ++w) {
+#pragma unroll
+        for (int s = 0; s < kDim / 32; ++s) q[w][s] ^= flip;
     }
     float top[RW], sum[RW];
     f32x4 o[kLatent / 16][RW];
@@ -181,10 +213,6 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
         for (int d = 0; d < kLatent / 16; ++d) o[d][w] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
 
-    const uint32_t keys = a.topK + (a.draftSlots != 0 ? a.draft : 0u);
-    const uint32_t allTiles = (keys + kTile - 1) / kTile;
-    const uint32_t tile0 = static_cast<uint32_t>(static_cast<uint64_t>(allTiles) * split / a.splits);
-    const uint32_t tile1 = static_cast<uint32_t>(static_cast<uint64_t>(allTiles) * (split + 1) / a.splits);
     const uint8_t *hot = reinterpret_cast<const uint8_t *>(a.hot) + req * a.reqStride * F::bytes;
     const uint32_t ldsTiles = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((KVX_LDS uint8_t *)tiles));
     const uint32_t ldsGroup = ldsTiles + wk * kBuffers * kTileBytes;
@@ -268,15 +296,11 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
 
     for (uint32_t c0 = tile0; c0 < tile1; c0 += kChunk) {
         const uint32_t chunk = min(static_cast<uint32_t>(kChunk), tile1 - c0);
-        __syncthreads();
-        for (uint32_t i = threadIdx.x; i < kChunk * kTile; i += kThreads) {
-            const uint32_t k = c0 * kTile + i;
-            int32_t slot = -1;
-            if (i < chunk * kTile && k < keys) {
-                slot = k < a.topK ? reinterpret_cast<const KVX_GLB int32_t *>(a.slots)[static_cast<uint64_t>(req) * a.topK + k]
-                                  : reinterpret_cast<const KVX_GLB int32_t *>(a.draftSlots)[static_cast<uint64_t>(req) * a.draft + k - a.topK];
-            }
-            rowOf[i] = hot_row(slot, req, a.reqStride, a.hotRows, a.overflowSlot) < 0 ? -1 : slot;
+        if (c0 != tile0) {
+            int32_t slots[kSlots];
+            readSlots(c0, slots);
+            __syncthreads();
+            lookUp(slots);
         }
         __syncthreads();
         const uint32_t steps = (chunk + WK - 1) / WK;
@@ -341,17 +365,25 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
             // The weights are exp2(score - top) for a top at most 2^8 below the
             // largest score so far: the output is scaled only when one rose by more.
             if (__any(rise)) {
+                float keep[RW];
+                bool any = false;                    // (nothing is there to scale at the first tile)
 #pragma unroll
                 for (int w = 0; w < RW; ++w) {
                     const float now = fmaxf(top[w], most[w]);
-                    const float keep = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top[w] - now);
+                    any = any || top[w] != -INFINITY;
+                    keep[w] = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top[w] - now);
                     top[w] = now;
-                    sum[w] *= keep;
+                }
+                if (__any(any)) {
 #pragma unroll
-                    for (int d = 0; d < kLatent / 16; ++d) {
-                        keep_in_acc(o[d][w]);
-                        o[d][w] *= keep;
-                        keep_in_acc(o[d][w]);
+                    for (int w = 0; w < RW; ++w) {
+                        sum[w] *= keep[w];
+#pragma unroll
+                        for (int d = 0; d < kLatent / 16; ++d) {
+                            keep_in_acc(o[d][w]);
+                            o[d][w] *= keep[w];
+                            keep_in_acc(o[d][w]);
+                        }
                     }
                 }
             }
@@ -463,6 +495,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
             }
         }
         __syncthreads();
+        // a group's output counts exp2(its maximum - the largest) times
 #pragma unroll
         for (int w = 0; w < RW; ++w) {
             float most = -INFINITY, all = 0.0f;
@@ -474,23 +507,11 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
                 const float *x = stat[g * WR + wr][w * 16 + col];
                 all += x[1] * __builtin_amdgcn_exp2f(x[0] - base);
             }
-            const float keep = __builtin_amdgcn_exp2f(top[w] - base);
-#pragma unroll
-            for (int d = 0; d < kLatent / 16; ++d) {
-                keep_in_acc(o[d][w]);
-                o[d][w] *= keep;
-                keep_in_acc(o[d][w]);
-            }
+            // ... and, where this is all of it, over the sum
+            const float whole = a.splits > 1 ? 1.0f : (all == 0.0f ? 0.0f : __builtin_amdgcn_rcpf(all));
+            if (grp == 0) weigh[wave][w * 16 + col] = __builtin_amdgcn_exp2f(top[w] - base) * whole;
             top[w] = most;
             sum[w] = all;
-        }
-        __syncthreads();
-        if (wk == 0 && grp == 0) {
-#pragma unroll
-            for (int w = 0; w < RW; ++w) {
-                stat[wr][w * 16 + col][0] = top[w];
-                stat[wr][w * 16 + col][1] = sum[w];
-            }
         }
         KVX_LDS float *join = (KVX_LDS float *)tiles;
 #pragma unroll
@@ -499,23 +520,27 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
             for (int d = 0; d < kJoinCols / 16; ++d) {
 #pragma unroll
                 for (int w = 0; w < RW; ++w) {
-                    *reinterpret_cast<KVX_LDS f32x4 *>(join + (wave * kRows + w * 16 + col) * kJoinStride + d * 16 + grp * 4) =
-                        o[round * (kJoinCols / 16) + d][w];
+                    f32x4 &x = o[round * (kJoinCols / 16) + d][w];
+                    keep_in_acc(x);
+                    *reinterpret_cast<KVX_LDS f32x4 *>(join + (wave * kRows + w * 16 + col) * kJoinStride + d * 16 + grp * 4) = x;
                 }
             }
             __syncthreads();
-            for (uint32_t i = threadIdx.x; i < WR * kRows * (kJoinCols / 4); i += kThreads) {
+#pragma unroll
+            for (int n = 0; n < WR * kRows * (kJoinCols / 4) / kThreads; ++n) {
+                const uint32_t i = threadIdx.x + n * kThreads;
                 const uint32_t c = i % (kJoinCols / 4), r = i / (kJoinCols / 4);
                 f32x4 x = {};
 #pragma unroll
-                for (int g = 0; g < WK; ++g) x += *reinterpret_cast<const KVX_LDS f32x4 *>(join + (g * WR * kRows + r) * kJoinStride + c * 4);
+                for (int g = 0; g < WK; ++g) {
+                    x += *reinterpret_cast<const KVX_LDS f32x4 *>(join + (g * WR * kRows + r) * kJoinStride + c * 4) *
+                         weigh[g * WR + r / kRows][r % kRows];
+                }
                 const uint32_t index = qt * WR * kRows + r;
-                const float all = stat[r / kRows][r % kRows][1];
                 if (index < queries) {
                     if (a.splits == 1) {
-                        const float inv = all == 0.0f ? 0.0f : 1.0f / all;
                         KVX_GLB T *out = reinterpret_cast<KVX_GLB T *>(a.out) + (row0 + index) * kLatent + round * kJoinCols + c * 4;
-                        *reinterpret_cast<KVX_GLB u32x2 *>(out) = u32x2{pack2<T>(x[0] * inv, x[1] * inv), pack2<T>(x[2] * inv, x[3] * inv)};
+                        *reinterpret_cast<KVX_GLB u32x2 *>(out) = u32x2{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3])};
                     } else {
                         KVX_GLB float *out = reinterpret_cast<KVX_GLB float *>(a.part) + ((static_cast<uint64_t>(req) * a.splits + split) * queries + index) * kLatent + round * kJoinCols + c * 4;
                         *reinterpret_cast<KVX_GLB f32x4 *>(out) = x;
@@ -529,7 +554,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
         for (int w = 0; w < RW; ++w) {
             if (query[w] >= queries) continue;
             if (a.splits == 1) {
-                const float inv = sum[w] == 0.0f ? 0.0f : 1.0f / sum[w];
+                const float inv = sum[w] == 0.0f ? 0.0f : __builtin_amdgcn_rcpf(sum[w]);
                 KVX_GLB T *out = reinterpret_cast<KVX_GLB T *>(a.out) + (row0 + query[w]) * kLatent + grp * 4;
 #pragma unroll
                 for (int d = 0; d < kLatent / 16; ++d) {
@@ -588,7 +613,7 @@ __global__ __launch_bounds__(kThreads) void kvx_tree_attention_join(AttnArgs a)
         x += v[0] * keep;
         y += v[1] * keep;
     }
-    const float inv = all == 0.0f ? 0.0f : 1.0f / all;
+    const float inv = all == 0.0f ? 0.0f : __builtin_amdgcn_rcpf(all);
     *reinterpret_cast<KVX_GLB u32x4 *>(reinterpret_cast<KVX_GLB T *>(a.out) + row * kLatent + lane * 8) =
         u32x4{pack2<T>(x[0] * inv, x[1] * inv), pack2<T>(x[2] * inv, x[3] * inv), pack2<T>(y[0] * inv, y[1] * inv), pack2<T>(y[2] * inv, y[3] * inv)};
     if (lane == 0 && a.lse != 0) {

@@ -502,14 +502,13 @@ void DoExportRows(const uint64_t *segBases, bool fused, uint32_t layer_id, uint3
 
 void CheckRowForm(const char *what, uint32_t latent, uint32_t rope, uint32_t dtype, uint32_t quant, bool codes)
 {
-    const std::string name(what);
     if (latent != static_cast<uint32_t>(kvx::kLatent) || rope != static_cast<uint32_t>(kvx::kRope)) {
-        throw Error(name + ": rows of kv_lora_rank 512 and qk_rope 64 are supported, got " + std::to_string(latent) +
+        throw Error(std::string(what) + ": rows of kv_lora_rank 512 and qk_rope 64 are supported, got " + std::to_string(latent) +
                     " and " + std::to_string(rope));
     }
-    if (dtype > KVX_DTYPE_FP16) throw Error(name + ": dtype must be bf16 or fp16");
-    if (quant > KVX_QUANT_ROW) throw Error(name + ": unknown row form");
-    if (codes && quant == KVX_QUANT_NONE) throw Error(name + ": rows of 16-bit values hold no codes");
+    if (dtype > KVX_DTYPE_FP16) throw Error(std::string(what) + ": dtype must be bf16 or fp16");
+    if (quant > KVX_QUANT_ROW) throw Error(std::string(what) + ": unknown row form");
+    if (codes && quant == KVX_QUANT_NONE) throw Error(std::string(what) + ": rows of 16-bit values hold no codes");
 }
 
 kvx::RowCopyArgs RowCopy(const char *what, uint64_t rows16, uint64_t rowStride, uint64_t hot, uint64_t hotRows,
@@ -525,10 +524,9 @@ kvx::RowCopyArgs RowCopy(const char *what, uint64_t rows16, uint64_t rowStride, 
     a.rows = static_cast<uint64_t>(numReqs) * rowsPerReq;
     a.perReq = rowsPerReq;
     a.overflowSlot = reinterpret_cast<uint64_t>(g.overflow);
-    const std::string name(what);
-    if (a.rows >= 1ull << 31) throw Error(name + ": num_reqs * rows_per_req must be below 2^31");
-    if (slots == 0 && a.rows > hotRows) throw Error(name + ": more rows than hot_rows and no slots");
-    if (a.rows != 0 && (rows16 == 0 || hot == 0)) throw Error(name + ": the rows must be device addresses");
+    if (a.rows >= 1ull << 31) throw Error(std::string(what) + ": num_reqs * rows_per_req must be below 2^31");
+    if (slots == 0 && a.rows > hotRows) throw Error(std::string(what) + ": more rows than hot_rows and no slots");
+    if (a.rows != 0 && (rows16 == 0 || hot == 0)) throw Error(std::string(what) + ": the rows must be device addresses");
     return a;
 }
 

@@ -26,6 +26,9 @@ import torch
 from ..kvops_ext import _kvops
 from .xds_offload import _stream_handle
 
+# the current stream's handle without a Stream object (a call of one decode step is a few microseconds)
+_current = torch._C._cuda_getCurrentRawStream
+
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _QUANTS = {"none": 0, "latent": 1, "row": 2}
 
@@ -68,39 +71,42 @@ def row_format(dtype=torch.bfloat16, kv_lora_rank: int = 512, qk_rope: int = 64,
 
 
 def _hot(fmt: RowFormat, hot: torch.Tensor) -> int:
-    """Rows of the hot buffer: a contiguous tensor, of any type, whose last
-    dimension is one row of bytes or which holds a whole number of rows."""
+    """Rows of the hot buffer: a contiguous tensor, of any type, that holds a
+    whole number of rows."""
     if not hot.is_cuda:
         raise ValueError("hot must be on the GPU")
     if not hot.is_contiguous():
         raise ValueError("hot must be contiguous")
-    nbytes = hot.numel() * hot.element_size()
-    if nbytes % fmt.row_bytes:
-        raise ValueError("hot holds {} bytes, no multiple of the row's {}".format(nbytes, fmt.row_bytes))
-    return nbytes // fmt.row_bytes
+    rows, rest = divmod(hot.nbytes, fmt.row_bytes)
+    if rest:
+        raise ValueError("hot holds {} bytes, no multiple of the row's {}".format(hot.nbytes, fmt.row_bytes))
+    return rows
 
 
-def _ints(x: torch.Tensor, name: str, shape, dtype, device) -> int:
-    if x.dtype is not dtype or x.shape != shape or not x.is_contiguous() or x.device != device:
-        raise ValueError("{} must be a contiguous {} tensor of shape {} on {}, got {} of {} on {}".format(
+def _address(x: torch.Tensor, name: str, shape, dtype, device: int) -> int:
+    if x.dtype is not dtype or x.shape != shape or not x.is_contiguous() or x.get_device() != device:
+        raise ValueError("{} must be a contiguous {} tensor of shape {} on cuda:{}, got {} of {} on {}".format(
             name, dtype, tuple(shape), device, x.dtype, tuple(x.shape), x.device))
     return x.data_ptr()
 
 
-def _slots(slots: Optional[torch.Tensor], rows: int, device) -> Tuple[int, int, int]:
+def _slots(slots: Optional[torch.Tensor], rows: int, device: int) -> Tuple[int, int, int]:
     """(address, requests, rows of each) of int32 slots [requests, rows]."""
     if slots is None:
         return 0, 1, rows
     if slots.dim() != 2 or slots.numel() != rows:
         raise ValueError("slots must be [requests, rows of each] with one slot for each of the {} rows, got {}".format(
             rows, tuple(slots.shape)))
-    return _ints(slots, "slots", slots.shape, torch.int32, device), slots.shape[0], slots.shape[1]
+    return _address(slots, "slots", slots.shape, torch.int32, device), slots.shape[0], slots.shape[1]
 
 
-def _stride(req_stride_rows: int) -> int:
+def _stream_of(stream, device: int) -> int:
+    return _current(device) if stream is None else _stream_handle(stream)
+
+
+def _check_stride(req_stride_rows: int) -> None:
     if req_stride_rows < 0:
         raise ValueError("req_stride_rows must not be negative")
-    return req_stride_rows
 
 
 def _needs_codes(fmt: RowFormat) -> None:
@@ -110,8 +116,8 @@ def _needs_codes(fmt: RowFormat) -> None:
 
 def quantize_rows(fmt: RowFormat, rows: torch.Tensor, hot: torch.Tensor, slots: Optional[torch.Tensor] = None,
                   req_stride_rows: int = 0, stream=None) -> None:
-    """Write 16-bit rows [..., dim] (``fmt.dtype``, contiguous but for a stride
-    of the next-to-last dimension) into hot rows of ``fmt``.  Row i goes to the
+    """Write 16-bit rows [..., dim] (``fmt.dtype``; contiguous, or one stride
+    between rows, a multiple of 8) into hot rows of ``fmt``.  Row i goes to the
     i-th of ``slots`` (int32 [requests, rows of each], negative: left out), or
     without slots to hot row i.  No two rows may name the same slot."""
     _needs_codes(fmt)
@@ -119,15 +125,19 @@ def quantize_rows(fmt: RowFormat, rows: torch.Tensor, hot: torch.Tensor, slots: 
         raise ValueError("rows must be {} [..., {}] on the GPU, got {} {}".format(
             fmt.dtype, fmt.dim, rows.dtype, tuple(rows.shape)))
     if rows.dim() != 2:
-        rows = rows.reshape(-1, fmt.dim)
-    if rows.stride(1) != 1 or rows.stride(0) % 8:
-        rows = rows.contiguous()
-    n, hot_rows = rows.shape[0], _hot(fmt, hot)
-    at, reqs, each = _slots(slots, n, rows.device)
+        rows = rows.view(-1, fmt.dim)      # (no copy: it would be made on the current stream, not on `stream`)
+    if rows.stride(1) != 1 or rows.stride(0) % 8 or rows.stride(0) < 0:
+        raise ValueError("rows must be contiguous but for a stride between them, a multiple of 8, got {}".format(
+            rows.stride()))
+    _check_stride(req_stride_rows)
+    n, hot_rows, device = rows.shape[0], _hot(fmt, hot), rows.get_device()
+    if hot.get_device() != device:
+        raise ValueError("hot must be on cuda:{}, as the rows are".format(device))
+    at, reqs, each = _slots(slots, n, device)
     if slots is None and n > hot_rows:
         raise ValueError("{} rows and no slots, but hot holds {}".format(n, hot_rows))
     _kvops.quantize_rows(rows.data_ptr(), rows.stride(0) * 2, hot.data_ptr(), hot_rows, at, reqs, each,
-                         _stride(req_stride_rows), *fmt.code, _stream_handle(stream))
+                         req_stride_rows, *fmt.code, _stream_of(stream, device))
 
 
 def dequantize_rows(fmt: RowFormat, hot: torch.Tensor, slots: Optional[torch.Tensor] = None,
@@ -143,15 +153,16 @@ def dequantize_rows(fmt: RowFormat, hot: torch.Tensor, slots: Optional[torch.Ten
         n = hot_rows if slots is None else slots.numel()
         out = torch.empty((n, fmt.dim), dtype=dtype or fmt.dtype, device=hot.device)
     elif (out.dtype not in _DTYPES or (dtype is not None and out.dtype is not dtype) or out.shape[-1] != fmt.dim or
-          not out.is_contiguous() or out.device != hot.device):
+          not out.is_contiguous() or out.get_device() != hot.get_device()):
         raise ValueError("out must be contiguous, of the dtype asked for, [rows, {}] on {}, got {} {} on {}".format(
             fmt.dim, hot.device, out.dtype, tuple(out.shape), out.device))
-    n = out.numel() // fmt.dim
-    at, reqs, each = _slots(slots, n, hot.device)
+    _check_stride(req_stride_rows)
+    n, device = out.numel() // fmt.dim, hot.get_device()
+    at, reqs, each = _slots(slots, n, device)
     if slots is None and n > hot_rows:
         raise ValueError("{} rows and no slots, but hot holds {}".format(n, hot_rows))
-    _kvops.dequantize_rows(hot.data_ptr(), hot_rows, at, reqs, each, _stride(req_stride_rows), out.data_ptr(),
-                           *fmt.code, _DTYPES[out.dtype], _stream_handle(stream))
+    _kvops.dequantize_rows(hot.data_ptr(), hot_rows, at, reqs, each, req_stride_rows, out.data_ptr(),
+                           *fmt.code, _DTYPES[out.dtype], _stream_of(stream, device))
     return out
 
 
@@ -183,28 +194,30 @@ def tree_attention(fmt: RowFormat, q: torch.Tensor, hot: torch.Tensor, slots: to
     if sd != 1 or (sb | st | sh) % 8 or min(sb, st, sh) < 0:
         raise ValueError("q's last dimension must be contiguous and its other strides multiples of 8, got {}".format(
             q.stride()))
-    device = q.device
-    hot_rows = _hot(fmt, hot)
+    _check_stride(req_stride_rows)
+    device, hot_rows = q.get_device(), _hot(fmt, hot)
+    if hot.get_device() != device:
+        raise ValueError("hot must be on cuda:{}, as the queries are".format(device))
     if slots.dim() != 2 or slots.shape[0] < reqs:
         raise ValueError("slots must be [requests, topK] with a row for each of the {} requests, got {}".format(
             reqs, tuple(slots.shape)))
-    at = _ints(slots, "slots", slots.shape, torch.int32, device)
+    at = _address(slots, "slots", slots.shape, torch.int32, device)
     d_at = m_at = 0
     if draft_slots is not None:
-        d_at = _ints(draft_slots, "draft_slots", (reqs, tokens), torch.int32, device)
+        d_at = _address(draft_slots, "draft_slots", (reqs, tokens), torch.int32, device)
         if tree_mask is not None:
-            m_at = _ints(tree_mask, "tree_mask", (reqs, tokens), torch.int64, device)
+            m_at = _address(tree_mask, "tree_mask", (reqs, tokens), torch.int64, device)
     elif tree_mask is not None:
         raise ValueError("tree_mask needs draft_slots")
     if out is None:
-        out = torch.empty((reqs, tokens, heads, fmt.kv_lora_rank), dtype=fmt.dtype, device=device)
+        out = torch.empty((reqs, tokens, heads, fmt.kv_lora_rank), dtype=fmt.dtype, device=q.device)
     else:
-        _ints(out, "out", (reqs, tokens, heads, fmt.kv_lora_rank), fmt.dtype, device)
+        _address(out, "out", (reqs, tokens, heads, fmt.kv_lora_rank), fmt.dtype, device)
     if lse is None:
-        lse = torch.empty((reqs, tokens, heads), dtype=torch.float32, device=device)
+        lse = torch.empty((reqs, tokens, heads), dtype=torch.float32, device=q.device)
     else:
-        _ints(lse, "lse", (reqs, tokens, heads), torch.float32, device)
+        _address(lse, "lse", (reqs, tokens, heads), torch.float32, device)
     _kvops.tree_attention(q.data_ptr(), sb * 2, st * 2, sh * 2, hot.data_ptr(), hot_rows, at, d_at, m_at,
                           out.data_ptr(), lse.data_ptr(), reqs, tokens, heads, slots.shape[1],
-                          _stride(req_stride_rows), softmax_scale, *fmt.code, _stream_handle(stream))
+                          req_stride_rows, softmax_scale, *fmt.code, _stream_of(stream, device))
     return out, lse

@@ -480,7 +480,7 @@ def test_refusals():
 
     rows = torch.zeros((4, 576), dtype=torch.bfloat16, device="cuda")
     for args in [(xds.row_format(torch.bfloat16), rows, v["hot"]), (fmt, rows.half(), v["hot"]), (fmt, rows[:, :512], v["hot"]),
-                 (fmt, rows.cpu(), v["hot"]), (fmt, rows, v["hot"][:2].contiguous()), (fmt, rows, v["hot"], v["slots"]),
+                 (fmt, torch.zeros((4, 580), dtype=torch.bfloat16, device="cuda")[:, :576], v["hot"]), (fmt, rows.cpu(), v["hot"]), (fmt, rows, v["hot"][:2].contiguous()), (fmt, rows, v["hot"], v["slots"]),
                  (fmt, rows, v["hot"], torch.zeros((2, 2), device="cuda", dtype=torch.int64))]:
         with pytest.raises(ValueError):
             xds.quantize_rows(*args)

@@ -22,7 +22,8 @@ OUT = os.path.join(HERE, "kvops_ext")
 INCLUDE = os.path.join(ROOT, "include")
 
 HIP_SOURCES = ["sieve.hip", "sieve_fast.hip", "sieve_wave.hip", "sieve_batch.hip", "sieve_table.hip", "rows.hip",
-               "quant_rows.hip", "attn.hip", "kvx_host.hip"]
+               "quant_rows.hip", "attn.hip", "attn_wide.hip",
+               "kvx_host.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 HIP_FLAGS = [

@@ -1,11 +1,15 @@
-// Attention of drafted tokens over the hot buffer (kvx/kvx_attn.h).
+// Attention of drafted tokens over the hot buffer (kvx/kvx_attn.h): few queries
+// a workgroup, the joining of workgroups that share a query's keys, and how a
+// call is cut up.  attn_wide.hip has the kernel for many queries.
 //
-// A workgroup of four waves takes up to 16 * RW * WR queries (node, head) of
-// one request and walks a range of the request's keys, the selected slots and
-// then the drafted tokens' own, 32 at a time.  A wave holds RW * 16 queries in
-// registers with their whole output (512 columns, 32 bits): WR waves share the
-// keys in LDS with queries of their own, and 4 / WR groups of waves take every
-// (4 / WR)-th tile of keys; their outputs are joined at the end.
+// Four waves take the same 16 queries (node, head) of a request, and each every
+// fourth tile of 32 keys of the workgroup's range, in LDS of its own: nothing
+// waits for another wave until their outputs are joined at the end.  The tile
+// that a wave loads next replaces the one it works on panel by panel, as the
+// output's products are done with each, so that a load is under way nearly all
+// the time; memory bounds this kernel, or, where several workgroups read the
+// same keys, the way from L2 to LDS (64 bytes a cycle: a wave's tile 576 cycles,
+// while the matrix unit needs 1088 and works for four waves at once).
 //
 // Scores are held transposed, S^T = K Q^T (keys down, queries across the
 // lanes), so that a lane's scores, its running maximum and its sum all belong
@@ -15,207 +19,65 @@
 // upper and 4 of its lower half for each group of 16 lanes.
 #include <algorithm>
 
-#include "row_format.h"
+#include "attn_tile.h"
 
 namespace kvx {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kTile = 32;                 // keys a tile
-constexpr int kPanels = kDim / 64;        // a row in LDS: 9 panels of 64 values (128 bytes)
-constexpr int kPanelBytes = kTile * 128;
-constexpr int kTileBytes = kPanels * kPanelBytes;
-constexpr int kChunk = 64;                // tiles whose rows are looked up at a time
+constexpr int kWaves = 4;
+constexpr int kRows = 16;                 // queries of a workgroup
 constexpr int kAhead = 2;                 // panels whose operands are read ahead
-constexpr float kRise = 8.0f;             // a maximum may rise by 2^8 before the output is scaled down again
 
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef float f32x2 __attribute__((ext_vector_type(2)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-#define KVX_LDS __attribute__((address_space(3)))
-#define KVX_GLB __attribute__((address_space(1)))
-
-// what a key without a row reads
-__device__ __align__(128) uint8_t kvx_no_row[kDim * 2];
-
-template <int DTYPE>
-struct Elem;
-template <>
-struct Elem<KVX_DTYPE_BF16> {
-    typedef __bf16 T;
-    static constexpr uint32_t special = 0x7F80u;   // exponent of infinities and NaN
-    static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c)
-    {
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c,
-                                                       0, 0, 0);
-    }
-    static __device__ __forceinline__ uint32_t from_codes(uint32_t codes, float scale, bool high)
-    {
-        return __builtin_bit_cast(uint32_t, high ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, true)
-                                                 : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, false));
-    }
-};
-template <>
-struct Elem<KVX_DTYPE_FP16> {
-    typedef _Float16 T;
-    static constexpr uint32_t special = 0x7C00u;
-    static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c)
-    {
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0,
-                                                      0, 0);
-    }
-    static __device__ __forceinline__ uint32_t from_codes(uint32_t codes, float scale, bool high)
-    {
-        return __builtin_bit_cast(uint32_t, high ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, scale, true)
-                                                 : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, scale, false));
-    }
-};
-
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float a, float b)
-{
-    typedef T T2 __attribute__((ext_vector_type(2)));
-    T2 v;
-    v[0] = static_cast<T>(a);
-    v[1] = static_cast<T>(b);
-    return __builtin_bit_cast(uint32_t, v);
-}
-
-// Over the four lanes that hold scores of one query (lane % 16).
-template <typename F>
-__device__ __forceinline__ float over_query(float x, F f)
-{
-    typedef unsigned int u2 __attribute__((ext_vector_type(2)));
-    u2 v = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    x = f(__uint_as_float(v[0]), __uint_as_float(v[1]));
-    v = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return f(__uint_as_float(v[0]), __uint_as_float(v[1]));
-}
-
-// The output stays in the accumulation registers: without this the compiler
-// keeps second copies of it around each place that scales it, and spills.
-__device__ __forceinline__ void keep_in_acc(f32x4 &x) { asm volatile("" : "+a"(x)); }
-
-// Byte of the 16-byte chunk c (0..7) of row r in a panel: rows one after
-// another are 128 bytes apart, so the chunks of 8 rows are permuted to spread a
-// column over the banks.
-__device__ __forceinline__ uint32_t chunk_at(uint32_t r, uint32_t c) { return r * 128u + ((c ^ (r & 7u)) << 4); }
-
-// 16 bytes a lane from memory to LDS at base + lane * 16, not waited for: the
-// caller counts the loads (wait_loads).
-__device__ __forceinline__ void load_to_lds(const uint8_t *from, uint32_t base)
-{
-    // (a wait state between the write of m0 and its use)
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(base) : "memory");
-}
-
-template <int LEFT>
-__device__ __forceinline__ void wait_loads()
-{
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LEFT) : "memory");
-}
-
-// Every wave's LDS reads are done and what it waited for is there.
-__device__ __forceinline__ void meet() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
-
-template <int DTYPE, int QUANT, int RW, int WR>
+template <int DTYPE, int QUANT>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))) void kvx_tree_attention(AttnArgs a)
 {
     typedef Elem<DTYPE> E;
     typedef typename E::T T;
     using F = RowForm<QUANT>;
     constexpr bool kCodes = QUANT != KVX_QUANT_NONE;
-    constexpr int WK = 4 / WR;                       // groups of waves that take keys of their own
-    constexpr int kRows = RW * 16;                   // queries of a wave
-    constexpr int kBuffers = kCodes ? (WR == 1 ? 1 : 2) : WR;   // of a group
-    constexpr int kGroups = 4 / WR;                  // groups of 8 rows that a wave loads
-    constexpr int kLoads = kGroups * kPanels;        // loads of a tile by a wave (16-bit rows)
-    constexpr int kJoinCols = kLatent / RW;
-    constexpr int kJoinStride = kJoinCols + 4;       // floats
-    constexpr int kJoinBytes = WK > 1 ? 4 * kRows * kJoinStride * 4 : 0;
-    constexpr int kTilesBytes = WK * kBuffers * kTileBytes;
+    constexpr int kRowGroups = kTile / 8;            // loads of 8 rows by 128 bytes for a panel
+    constexpr int kJoinStride = kLatent + 4;         // floats
 
-    __shared__ __align__(128) uint8_t tiles[kTilesBytes > kJoinBytes ? kTilesBytes : kJoinBytes];
+    __shared__ __align__(128) uint8_t tiles[kWaves * kTileBytes];    // and, at the end, the waves' outputs
     __shared__ int32_t rowOf[kChunk * kTile];        // hot row within the request of each key, -1: none
-    __shared__ float stat[4][kRows][2], weigh[4][kRows];
+    __shared__ float stat[kWaves][kRows][2], share[kWaves][kRows];
+    static_assert(kWaves * kRows * kJoinStride * 4 <= kWaves * kTileBytes, "outputs fit the tiles");
 
     const uint32_t lane = threadIdx.x & 63u;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t col = lane & 15u, grp = lane >> 4;
-    const uint32_t wr = wave % WR, wk = wave / WR;
     const uint32_t queries = a.draft * a.heads;
+    const AttnItem item(a);
+    if (!item.real) return;
+    const uint32_t req = item.req;
 
-    // consecutive workgroups of one XCD's share take the same keys
-    const uint32_t total = a.reqs * a.splits * a.queryTiles, share = (total + 7u) / 8u;
-    const uint32_t item = (blockIdx.x & 7u) * share + (blockIdx.x >> 3);
-    if ((blockIdx.x >> 3) >= share || item >= total) return;
-    const uint32_t qt = item % a.queryTiles, split = item / a.queryTiles % a.splits;
-    const uint32_t req = item / a.queryTiles / a.splits;
-
-    const uint32_t keys = a.topK + (a.draftSlots != 0 ? a.draft : 0u);
-    const uint32_t allTiles = (keys + kTile - 1) / kTile;
-    const uint32_t tile0 = static_cast<uint32_t>(static_cast<uint64_t>(allTiles) * split / a.splits);
-    const uint32_t tile1 = static_cast<uint32_t>(static_cast<uint64_t>(allTiles) * (split + 1) / a.splits);
-    // slots of the chunk from tile c0 on, kThreads apart (-1 past the range)
-    constexpr int kSlots = kChunk * kTile / kThreads;
-    auto readSlots = [&](uint32_t c0, int32_t (&slot)[kSlots]) {
-#pragma unroll
-        for (int n = 0; n < kSlots; ++n) {
-            const uint32_t k = c0 * kTile + n * kThreads + threadIdx.x;
-            slot[n] = -1;
-            if (k < min(keys, tile1 * kTile)) {
-                slot[n] = k < a.topK ? reinterpret_cast<const KVX_GLB int32_t *>(a.slots)[static_cast<uint64_t>(req) * a.topK + k]
-                                     : reinterpret_cast<const KVX_GLB int32_t *>(a.draftSlots)[static_cast<uint64_t>(req) * a.draft + k - a.topK];
-            }
-        }
-    };
-    auto lookUp = [&](const int32_t (&slot)[kSlots]) {
-#pragma unroll
-        for (int n = 0; n < kSlots; ++n) {
-            rowOf[n * kThreads + threadIdx.x] = hot_row(slot[n], req, a.reqStride, a.hotRows, a.overflowSlot) < 0 ? -1 : slot[n];
-        }
-    };
     int32_t firstSlots[kSlots];
-    readSlots(tile0, firstSlots);                    // (before the queries: the rows' addresses wait for them)
+    read_slots(a, item, item.tile0, firstSlots);     // (before the queries: the rows' addresses wait for them)
 
-    uint32_t query[RW];
-    u32x4 q[RW][kDim / 32];
-    uint64_t sees[RW];                               // drafted tokens that the query sees
-#pragma unroll
-    for (int w = 0; w < RW; ++w) {
-        query[w] = (qt * WR + wr) * kRows + w * 16 + col;
-        const uint32_t real = min(query[w], queries - 1);      // (what lies past the last query is not stored)
+    const uint32_t query = item.queryTile * kRows + col;             // this lane's
+    u32x4 q[kDim / 32];
+    uint64_t sees;                                   // drafted tokens that the query sees
+    {
+        const uint32_t real = min(query, queries - 1);               // (what lies past the last query is not stored)
         const uint32_t node = real / a.heads, head = real % a.heads;
         const uint64_t at = a.q + req * a.qStrideB + node * a.qStrideT + head * a.qStrideH + grp * 16;
 #pragma unroll
-        for (int s = 0; s < kDim / 32; ++s) q[w][s] = *reinterpret_cast<const KVX_GLB u32x4 *>(at + s * 64);
-        sees[w] = a.treeMask != 0 ? reinterpret_cast<const KVX_GLB uint64_t *>(a.treeMask)[req * a.draft + node]
-                                  : ~0ull >> (63u - node);
+        for (int s = 0; s < kDim / 32; ++s) q[s] = *reinterpret_cast<const KVX_GLB u32x4 *>(at + s * 64);
+        sees = a.treeMask != 0 ? reinterpret_cast<const KVX_GLB uint64_t *>(a.treeMask)[req * a.draft + node]
+                               : ~0ull >> (63u - node);
     }
-    lookUp(firstSlots);
+    look_up(a, item, firstSlots, rowOf);
     const uint32_t flip = a.negate ? 0x80008000u : 0u;               // a negative scale: negative queries
 #pragma unroll
-    for (int w = 0; w < RW; ++w) {
+    for (int s = 0; s < kDim / 32; ++s) q[s] ^= flip;
+    float top = -INFINITY, sum = 0.0f;
+    f32x4 o[kLatent / 16];
 #pragma unroll
-        for (int s = 0; s < kDim / 32; ++s) q[w][s] ^= flip;
-    }
-    float top[RW], sum[RW];
-    f32x4 o[kLatent / 16][RW];
-#pragma unroll
-    for (int w = 0; w < RW; ++w) {
-        top[w] = -INFINITY;
-        sum[w] = 0.0f;
-#pragma unroll
-        for (int d = 0; d < kLatent / 16; ++d) o[d][w] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    }
+    for (int d = 0; d < kLatent / 16; ++d) o[d] = f32x4{};
 
     const uint8_t *hot = reinterpret_cast<const uint8_t *>(a.hot) + req * a.reqStride * F::bytes;
-    const uint32_t ldsTiles = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((KVX_LDS uint8_t *)tiles));
-    const uint32_t ldsGroup = ldsTiles + wk * kBuffers * kTileBytes;
+    const uint32_t ldsTile = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((KVX_LDS uint8_t *)tiles)) + wave * kTileBytes;
+    const KVX_LDS uint8_t *tile = (KVX_LDS uint8_t *)(uintptr_t)ldsTile;
     // this lane's bytes of a tile: its key's chunk for a score step (two steps
     // a panel), and its four columns of four keys for an output step
     const uint32_t atKey[2] = {chunk_at(col, grp), chunk_at(col, grp + 4)};
@@ -224,65 +86,56 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
     for (int d = 0; d < 4; ++d) atValue[d] = chunk_at(grp * 4 + (col >> 2), d * 2 + ((col & 3u) >> 1)) + (col & 1u) * 8u;
 
     // ---- bringing a tile in ----
-    // 16-bit rows: straight to LDS, 8 rows by 128 bytes a load
-    auto fetch = [&](uint32_t t, uint32_t buffer) {
-#pragma unroll
-        for (int g = 0; g < kGroups; ++g) {
-            const uint32_t r = (wr * kGroups + g) * 8 + (lane >> 3);
-            const int32_t row = rowOf[t * kTile + r];
-            const uint8_t *from = row < 0 ? kvx_no_row : hot + static_cast<uint64_t>(static_cast<uint32_t>(row)) * F::bytes;
-            from += ((lane & 7u) ^ (lane >> 3)) * 16;
-#pragma unroll
-            for (int p = 0; p < kPanels; ++p) {
-                load_to_lds(from + p * 128, ldsGroup + buffer * kTileBytes + p * kPanelBytes + (wr * kGroups + g) * 1024);
-            }
-        }
+    auto rowStart = [&](uint32_t t, uint32_t r) {
+        const int32_t row = rowOf[t * kTile + r];
+        return row < 0 ? kvx_no_row : hot + static_cast<uint64_t>(static_cast<uint32_t>(row)) * F::bytes;
     };
+    // 16-bit rows: straight to LDS, 8 rows by 128 bytes a load; the panels in the order in which they are used
+    const uint8_t *from[kRowGroups];
+    auto sources = [&](uint32_t t) {
+#pragma unroll
+        for (int g = 0; g < kRowGroups; ++g) from[g] = rowStart(t, g * 8 + (lane >> 3)) + ((lane & 7u) ^ (lane >> 3)) * 16;
+    };
+    auto loadPanel = [&](int p) {
+#pragma unroll
+        for (int g = 0; g < kRowGroups; ++g) load_panel(from[g], p, ldsTile + p * kPanelBytes + g * 1024);
+    };
+    constexpr int kFirst = kPanels - 1;              // the rotary panel: scores alone use it
+    auto panelAt = [](int n) { return n == 0 ? kFirst : n - 1; };
     // 8-bit rows: through registers, 16 rows by a panel of 64 codes a load
-    constexpr int kParts = WR == 1 ? 2 : 1;          // halves of the tile's rows that a wave brings in
-    constexpr int kStep = WR == 4 ? 2 : 1;           // ... and every how many panels
     constexpr int kCodePanels = F::codes / 64;
-    constexpr int kHeld = (kPanels + kStep - 1) / kStep;
-    u32x4 held[kParts][kHeld], rawHigh[kParts], scaleLow[kParts];
-    uint32_t scaleHigh[kParts];
-    const uint32_t firstPanel = WR == 4 ? wr >> 1 : 0u;
+    u32x4 held[2][kPanels], rawHigh[2], scaleLow[2];
+    uint32_t scaleHigh[2];
     const uint32_t j4 = lane & 3u;
     auto load = [&](uint32_t t) {
 #pragma unroll
-        for (int h = 0; h < kParts; ++h) {
-            const uint32_t r = (WR == 1 ? h : wr & 1u) * 16 + (lane >> 2);
-            const int32_t row = rowOf[t * kTile + r];
-            const uint64_t at = reinterpret_cast<uint64_t>(row < 0 ? kvx_no_row : hot + static_cast<uint64_t>(static_cast<uint32_t>(row)) * F::bytes);
+        for (int h = 0; h < 2; ++h) {
+            const uint64_t at = reinterpret_cast<uint64_t>(rowStart(t, h * 16 + (lane >> 2)));
 #pragma unroll
-            for (int i = 0; i < kHeld; ++i) {
-                const uint32_t p = i * kStep + firstPanel;
-                if (i * kStep + kStep > kPanels && p >= kPanels) continue;
+            for (int p = 0; p < kPanels; ++p) {
                 // (a panel kept in 16 bits: 32 bytes a lane)
-                const uint64_t from = at + p * 64 + (F::raw != 0 && p == kCodePanels ? j4 * 32 : j4 * 16);
-                held[h][i] = *reinterpret_cast<const KVX_GLB u32x4 *>(from);
-                if (F::raw != 0 && p == kCodePanels) rawHigh[h] = *reinterpret_cast<const KVX_GLB u32x4 *>(from + 16);
+                const uint64_t x = at + p * 64 + (F::raw != 0 && p == kCodePanels ? j4 * 32 : j4 * 16);
+                held[h][p] = *reinterpret_cast<const KVX_GLB u32x4 *>(x);
+                if (F::raw != 0 && p == kCodePanels) rawHigh[h] = *reinterpret_cast<const KVX_GLB u32x4 *>(x + 16);
             }
             scaleLow[h] = *reinterpret_cast<const KVX_GLB u32x4 *>(at + F::scaleAt);
             if (F::scales > 16) scaleHigh[h] = *reinterpret_cast<const KVX_GLB uint32_t *>(at + F::scaleAt + 16);
         }
     };
-    auto store = [&](uint32_t buffer) {
+    auto store = [&] {
 #pragma unroll
-        for (int h = 0; h < kParts; ++h) {
-            const uint32_t r = (WR == 1 ? h : wr & 1u) * 16 + (lane >> 2);
-            const uint32_t base = ldsGroup + buffer * kTileBytes;
-            const uint32_t low = base + chunk_at(r, j4 * 2), high = base + chunk_at(r, j4 * 2 + 1);
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t r = h * 16 + (lane >> 2);
+            const uint32_t low = ldsTile + chunk_at(r, j4 * 2), high = ldsTile + chunk_at(r, j4 * 2 + 1);
             const uint32_t shift = (j4 >> 1) * 8;
 #pragma unroll
-            for (int i = 0; i < kHeld; ++i) {
-                const uint32_t p = i * kStep + firstPanel;
-                if (i * kStep + kStep > kPanels && p >= kPanels) continue;
-                u32x4 x = held[h][i], y = rawHigh[h];
+            for (int p = 0; p < kPanels; ++p) {
+                u32x4 x = held[h][p], y = rawHigh[h];
                 if (F::raw == 0 || p != kCodePanels) {
                     // panel p's two groups: bytes 2p and 2p + 1
-                    const uint32_t four = i * kStep / 2 < 4 ? scaleLow[h][i * kStep / 2] : scaleHigh[h];
-                    const float scale = __uint_as_float(((four >> ((p & 1u) * 16 + shift)) & 255u) << 23);
-                    const u32x4 c = held[h][i];
+                    const uint32_t four = p < 8 ? scaleLow[h][p / 2 & 3] : scaleHigh[h];
+                    const float scale = __uint_as_float(((four >> ((p & 1) * 16 + shift)) & 255u) << 23);
+                    const u32x4 c = held[h][p];
                     x = u32x4{E::from_codes(c[0], scale, false), E::from_codes(c[0], scale, true),
                               E::from_codes(c[1], scale, false), E::from_codes(c[1], scale, true)};
                     y = u32x4{E::from_codes(c[2], scale, false), E::from_codes(c[2], scale, true),
@@ -294,115 +147,96 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
         }
     };
 
-    for (uint32_t c0 = tile0; c0 < tile1; c0 += kChunk) {
-        const uint32_t chunk = min(static_cast<uint32_t>(kChunk), tile1 - c0);
-        if (c0 != tile0) {
+    for (uint32_t c0 = item.tile0; c0 < item.tile1; c0 += kChunk) {
+        const uint32_t chunk = min(static_cast<uint32_t>(kChunk), item.tile1 - c0);
+        if (c0 != item.tile0) {
             int32_t slots[kSlots];
-            readSlots(c0, slots);
+            read_slots(a, item, c0, slots);
             __syncthreads();
-            lookUp(slots);
+            look_up(a, item, slots, rowOf);
         }
         __syncthreads();
-        const uint32_t steps = (chunk + WK - 1) / WK;
-
-        // tile i * WK + wk of the chunk, in its buffer
-        auto work = [&](uint32_t i, uint32_t buffer) {
-            const uint32_t t = min(i * WK + wk, static_cast<uint32_t>(kChunk - 1));
-            const bool past = i * WK + wk >= chunk;
-            const uint32_t live = past ? 0u : static_cast<uint32_t>(__ballot(rowOf[t * kTile + (lane & 31u)] >= 0));
+        if (wave < chunk) {
+            if constexpr (kCodes) {
+                load(wave);
+            } else {
+                sources(wave);
+#pragma unroll
+                for (int n = 0; n < kPanels; ++n) loadPanel(panelAt(n));
+            }
+        }
+        for (uint32_t t = wave; t < chunk; t += kWaves) {
+            const bool more = t + kWaves < chunk;
+            const uint32_t live = static_cast<uint32_t>(__ballot(rowOf[t * kTile + (lane & 31u)] >= 0));
             const uint32_t k0 = (c0 + t) * kTile;
-            // (the same for every wave of the workgroup)
-            const bool drafted = (c0 + i * WK + WK) * kTile > a.topK && a.draftSlots != 0;
-            if (live == 0 && !(drafted && WR > 1)) return;
-            const KVX_LDS uint8_t *tile = (KVX_LDS uint8_t *)(uintptr_t)(ldsGroup + buffer * kTileBytes);
+            const bool drafted = k0 + kTile > a.topK && a.draftSlots != 0;
+            if constexpr (kCodes) {
+                store();
+                if (more) load(t + kWaves);
+            }
 
             // the operands of the next panels are on their way while one panel's are multiplied
-            f32x4 s[2][RW] = {};
+            f32x4 s[2] = {};
             u32x4 key[kAhead + 1][4];
-            auto readKeys = [&](int p) {
+            auto readKeys = [&](int n) {
+                if constexpr (!kCodes) wait_panels(kPanels - 1 - n);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    key[p % (kAhead + 1)][i] = *reinterpret_cast<const KVX_LDS u32x4 *>(tile + atKey[i >> 1] + p * kPanelBytes + (i & 1) * 2048);
+                    key[n % (kAhead + 1)][i] = *reinterpret_cast<const KVX_LDS u32x4 *>(
+                        tile + atKey[i >> 1] + panelAt(n) * kPanelBytes + (i & 1) * 2048);
                 }
             };
 #pragma unroll
-            for (int p = 0; p < kAhead; ++p) readKeys(p);
+            for (int n = 0; n < kAhead; ++n) readKeys(n);
 #pragma unroll
-            for (int p = 0; p < kPanels; ++p) {
-                if (p + kAhead < kPanels) readKeys(p + kAhead);
+            for (int n = 0; n < kPanels; ++n) {
+                if (n + kAhead < kPanels) readKeys(n + kAhead);
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-#pragma unroll
-                    for (int w = 0; w < RW; ++w) s[i & 1][w] = E::mfma(key[p % (kAhead + 1)][i], q[w][p * 2 + (i >> 1)], s[i & 1][w]);
-                }
+                for (int i = 0; i < 4; ++i) s[i & 1] = E::mfma(key[n % (kAhead + 1)][i], q[panelAt(n) * 2 + (i >> 1)], s[i & 1]);
                 __builtin_amdgcn_sched_barrier(0);
+            }
+            if (!kCodes && more) {
+                sources(t + kWaves);
+                loadPanel(kFirst);
             }
             if (live != ~0u || drafted) {
                 const uint32_t selected = k0 >= a.topK ? 0u : (a.topK - k0 >= 32u ? ~0u : (1u << (a.topK - k0)) - 1u);
+                uint32_t own = 0;                    // drafted tokens' bits of this tile
+                if (drafted) own = static_cast<uint32_t>(k0 >= a.topK ? sees >> (k0 - a.topK) : sees << min(a.topK - k0, 63u));
+                const uint32_t seen = (live & (selected | (own & ~selected))) >> (grp * 4);
 #pragma unroll
-                for (int w = 0; w < RW; ++w) {
-                    uint32_t own = 0;                // drafted tokens' bits of this tile
-                    if (drafted) own = static_cast<uint32_t>(k0 >= a.topK ? sees[w] >> (k0 - a.topK) : sees[w] << min(a.topK - k0, 63u));
-                    const uint32_t seen = (live & (selected | (own & ~selected))) >> (grp * 4);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const bool is = (seen & (1u << ((j >> 2) * 16 + (j & 3)))) != 0;
-                        s[j >> 2][w][j & 3] = is ? s[j >> 2][w][j & 3] : -INFINITY;
-                    }
+                for (int j = 0; j < 8; ++j) {
+                    const bool is = (seen & (1u << ((j >> 2) * 16 + (j & 3)))) != 0;
+                    s[j >> 2][j & 3] = is ? s[j >> 2][j & 3] : -INFINITY;
                 }
             }
-            float most[RW];
-            bool rise = false;
+            float most = s[0][0];                    // (a NaN is left out; its weight is one)
 #pragma unroll
-            for (int w = 0; w < RW; ++w) {
-                float m = s[0][w][0];                // (a NaN is left out; its weight is one)
-#pragma unroll
-                for (int j = 1; j < 8; ++j) m = fmaxf(m, s[j >> 2][w][j & 3]);
-                most[w] = over_query(m, [](float x, float y) { return fmaxf(x, y); }) * a.scaleLog2;
-                rise = rise || most[w] > top[w] + kRise;
-            }
+            for (int j = 1; j < 8; ++j) most = fmaxf(most, s[j >> 2][j & 3]);
+            most = over_query<4>(most, [](float x, float y) { return fmaxf(x, y); }) * a.scaleLog2;
             // The weights are exp2(score - top) for a top at most 2^8 below the
             // largest score so far: the output is scaled only when one rose by more.
-            if (__any(rise)) {
-                float keep[RW];
-                bool any = false;                    // (nothing is there to scale at the first tile)
-#pragma unroll
-                for (int w = 0; w < RW; ++w) {
-                    const float now = fmaxf(top[w], most[w]);
-                    any = any || top[w] != -INFINITY;
-                    keep[w] = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top[w] - now);
-                    top[w] = now;
-                }
+            if (__any(most > top + kRise)) {
+                const float now = fmaxf(top, most);
+                const bool any = top != -INFINITY;   // (nothing is there to scale at the first tile)
+                const float keep = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top - now);
+                top = now;
                 if (__any(any)) {
+                    sum *= keep;
 #pragma unroll
-                    for (int w = 0; w < RW; ++w) {
-                        sum[w] *= keep[w];
-#pragma unroll
-                        for (int d = 0; d < kLatent / 16; ++d) {
-                            keep_in_acc(o[d][w]);
-                            o[d][w] *= keep[w];
-                            keep_in_acc(o[d][w]);
-                        }
+                    for (int d = 0; d < kLatent / 16; ++d) {
+                        keep_in_acc(o[d]);
+                        o[d] *= keep;
+                        keep_in_acc(o[d]);
                     }
                 }
             }
-            // A drafted row that holds a NaN or an infinity must not reach the
-            // queries that do not see it, whose weight 0 would turn it into a NaN;
-            // those that see it have a score that is one already.
             if (drafted) {
-                if (WR > 1) meet();
-                constexpr uint32_t kWords = kTile * kLatent / 2;
-                for (uint32_t i2 = wr * 64 + lane; i2 < kWords; i2 += WR * 64) {
-                    const uint32_t r = i2 / (kLatent / 2), c = i2 % (kLatent / 2);
-                    if (k0 + r < a.topK) continue;
-                    KVX_LDS uint32_t *v = (KVX_LDS uint32_t *)(tile + (c >> 5) * kPanelBytes + chunk_at(r, (c >> 2) & 7u) + (c & 3u) * 4u);
-                    uint32_t x = *v;
-                    if ((x & E::special) == E::special) x &= 0xFFFF0000u;
-                    if ((x & (E::special << 16)) == (E::special << 16)) x &= 0xFFFFu;
-                    *v = x;
+                const uint32_t last = min(item.keys - k0, static_cast<uint32_t>(kTile));
+                for (uint32_t r = k0 >= a.topK ? 0u : a.topK - k0; r < last; ++r) {
+                    clean_row<DTYPE>(ldsTile, lane, chunk_at(r, lane & 7u));
                 }
-                if (WR > 1) meet();
             }
             u32x4 value[kAhead + 1][4];
             auto readValues = [&](int p) {
@@ -416,174 +250,75 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
             };
 #pragma unroll
             for (int p = 0; p < kAhead; ++p) readValues(p);
-            u32x4 weight[RW];
+            const float base = top == -INFINITY ? 0.0f : top;
+            float w[8];
 #pragma unroll
-            for (int w = 0; w < RW; ++w) {
-                const float base = top[w] == -INFINITY ? 0.0f : top[w];
-                float p[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j >> 2][w][j & 3], a.scaleLog2, -base));
-                    sum[w] += p[j];
-                }
-                weight[w] = u32x4{pack2<T>(p[0], p[1]), pack2<T>(p[2], p[3]), pack2<T>(p[4], p[5]), pack2<T>(p[6], p[7])};
+            for (int j = 0; j < 8; ++j) {
+                w[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j >> 2][j & 3], a.scaleLog2, -base));
+                sum += w[j];
             }
+            const u32x4 weight = {pack2<T>(w[0], w[1]), pack2<T>(w[2], w[3]), pack2<T>(w[4], w[5]), pack2<T>(w[6], w[7])};
 #pragma unroll
             for (int p = 0; p < kLatent / 64; ++p) {
                 if (p + kAhead < kLatent / 64) readValues(p + kAhead);
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-#pragma unroll
-                    for (int w = 0; w < RW; ++w) o[p * 4 + i][w] = E::mfma(value[p % (kAhead + 1)][i], weight[w], o[p * 4 + i][w]);
-                }
+                for (int i = 0; i < 4; ++i) o[p * 4 + i] = E::mfma(value[p % (kAhead + 1)][i], weight, o[p * 4 + i]);
                 __builtin_amdgcn_sched_barrier(0);
+                if (!kCodes && more) loadPanel(p);       // (the panel has been read: its products have begun)
             }
-        };
+        }
+    }
 
-        if constexpr (!kCodes && WR > 1) {
-            // a tile's loads are under way while kBuffers - 1 others are worked on
-            for (uint32_t i = 0; i + 1 < kBuffers && i < steps; ++i) fetch(i * WK + wk, i);
-            uint32_t buffer = 0, next = kBuffers - 1;
-            for (uint32_t i = 0; i < steps; ++i) {
-                if (i + kBuffers - 2 < steps - 1) wait_loads<(kBuffers - 2) * kLoads>();
-                else wait_loads<0>();
-                meet();
-                if (i + kBuffers - 1 < steps) fetch((i + kBuffers - 1) * WK + wk, next);
-                work(i, buffer);
-                buffer = buffer + 1 == kBuffers ? 0 : buffer + 1;
-                next = next + 1 == kBuffers ? 0 : next + 1;
-            }
-        } else if constexpr (!kCodes) {
-            for (uint32_t i = 0; i < steps; ++i) {
-                if (i * WK + wk >= chunk) break;
-                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // (the tile before has been read)
-                fetch(i * WK + wk, 0);
-                wait_loads<0>();
-                work(i, 0);
-            }
-        } else if constexpr (WR == 1) {
-            if (wk < chunk) load(wk);
-            for (uint32_t t = wk; t < chunk; t += WK) {
-                store(0);
-                if (t + WK < chunk) load(t + WK);
-                work(t / WK, 0);
-            }
+    // ---- joining the waves ----
+    sum = over_query<4>(sum, [](float x, float y) { return x + y; });
+    if (grp == 0) {
+        stat[wave][col][0] = top;
+        stat[wave][col][1] = sum;
+    }
+    __syncthreads();
+    // a wave's output counts exp2(its maximum - the largest) times
+    float all = 0.0f, most = -INFINITY;
+#pragma unroll
+    for (int g = 0; g < kWaves; ++g) most = fmaxf(most, stat[g][col][0]);
+    const float base = most == -INFINITY ? 0.0f : most;
+#pragma unroll
+    for (int g = 0; g < kWaves; ++g) all += stat[g][col][1] * __builtin_amdgcn_exp2f(stat[g][col][0] - base);
+    // ... and, where this is all of it, over the sum
+    const float whole = a.splits > 1 ? 1.0f : (all == 0.0f ? 0.0f : __builtin_amdgcn_rcpf(all));
+    if (grp == 0) share[wave][col] = __builtin_amdgcn_exp2f(top - base) * whole;
+    KVX_LDS float *join = (KVX_LDS float *)tiles;
+#pragma unroll
+    for (int d = 0; d < kLatent / 16; ++d) {
+        keep_in_acc(o[d]);
+        *reinterpret_cast<KVX_LDS f32x4 *>(join + (wave * kRows + col) * kJoinStride + d * 16 + grp * 4) = o[d];
+    }
+    __syncthreads();
+    const uint64_t row0 = static_cast<uint64_t>(req) * queries;      // first output row of the request
+    const uint64_t part0 = (static_cast<uint64_t>(req) * a.splits + item.split) * queries;
+#pragma unroll
+    for (int n = 0; n < kRows * (kLatent / 4) / kThreads; ++n) {
+        const uint32_t i = threadIdx.x + n * kThreads, c = i % (kLatent / 4), r = i / (kLatent / 4);
+        f32x4 x = {};
+#pragma unroll
+        for (int g = 0; g < kWaves; ++g) {
+            x += *reinterpret_cast<const KVX_LDS f32x4 *>(join + (g * kRows + r) * kJoinStride + c * 4) * share[g][r];
+        }
+        const uint32_t index = item.queryTile * kRows + r;
+        if (index >= queries) continue;
+        if (a.splits == 1) {
+            *reinterpret_cast<KVX_GLB u32x2 *>(reinterpret_cast<KVX_GLB T *>(a.out) + (row0 + index) * kLatent + c * 4) =
+                u32x2{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3])};
         } else {
-            load(wk);
-            store(0);
-            if (steps > 1) load(WK + wk);
-            for (uint32_t i = 0; i < steps; ++i) {
-                meet();
-                if (i + 1 < steps) store((i + 1) & 1u);
-                if (i + 2 < steps) load((i + 2) * WK + wk);
-                work(i, i & 1u);
-            }
+            *reinterpret_cast<KVX_GLB f32x4 *>(reinterpret_cast<KVX_GLB float *>(a.part) + (part0 + index) * kLatent + c * 4) = x;
         }
     }
-
-    // ---- joining the groups of waves ----
-#pragma unroll
-    for (int w = 0; w < RW; ++w) sum[w] = over_query(sum[w], [](float x, float y) { return x + y; });
-    const uint64_t row0 = static_cast<uint64_t>(req) * queries;        // first output row of the request
-    if constexpr (WK > 1) {
-        if (grp == 0) {
-#pragma unroll
-            for (int w = 0; w < RW; ++w) {
-                stat[wave][w * 16 + col][0] = top[w];
-                stat[wave][w * 16 + col][1] = sum[w];
-            }
-        }
-        __syncthreads();
-        // a group's output counts exp2(its maximum - the largest) times
-#pragma unroll
-        for (int w = 0; w < RW; ++w) {
-            float most = -INFINITY, all = 0.0f;
-#pragma unroll
-            for (int g = 0; g < WK; ++g) most = fmaxf(most, stat[g * WR + wr][w * 16 + col][0]);
-            const float base = most == -INFINITY ? 0.0f : most;
-#pragma unroll
-            for (int g = 0; g < WK; ++g) {
-                const float *x = stat[g * WR + wr][w * 16 + col];
-                all += x[1] * __builtin_amdgcn_exp2f(x[0] - base);
-            }
-            // ... and, where this is all of it, over the sum
-            const float whole = a.splits > 1 ? 1.0f : (all == 0.0f ? 0.0f : __builtin_amdgcn_rcpf(all));
-            if (grp == 0) weigh[wave][w * 16 + col] = __builtin_amdgcn_exp2f(top[w] - base) * whole;
-            top[w] = most;
-            sum[w] = all;
-        }
-        KVX_LDS float *join = (KVX_LDS float *)tiles;
-#pragma unroll
-        for (int round = 0; round < RW; ++round) {
-#pragma unroll
-            for (int d = 0; d < kJoinCols / 16; ++d) {
-#pragma unroll
-                for (int w = 0; w < RW; ++w) {
-                    f32x4 &x = o[round * (kJoinCols / 16) + d][w];
-                    keep_in_acc(x);
-                    *reinterpret_cast<KVX_LDS f32x4 *>(join + (wave * kRows + w * 16 + col) * kJoinStride + d * 16 + grp * 4) = x;
-                }
-            }
-            __syncthreads();
-#pragma unroll
-            for (int n = 0; n < WR * kRows * (kJoinCols / 4) / kThreads; ++n) {
-                const uint32_t i = threadIdx.x + n * kThreads;
-                const uint32_t c = i % (kJoinCols / 4), r = i / (kJoinCols / 4);
-                f32x4 x = {};
-#pragma unroll
-                for (int g = 0; g < WK; ++g) {
-                    x += *reinterpret_cast<const KVX_LDS f32x4 *>(join + (g * WR * kRows + r) * kJoinStride + c * 4) *
-                         weigh[g * WR + r / kRows][r % kRows];
-                }
-                const uint32_t index = qt * WR * kRows + r;
-                if (index < queries) {
-                    if (a.splits == 1) {
-                        KVX_GLB T *out = reinterpret_cast<KVX_GLB T *>(a.out) + (row0 + index) * kLatent + round * kJoinCols + c * 4;
-                        *reinterpret_cast<KVX_GLB u32x2 *>(out) = u32x2{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3])};
-                    } else {
-                        KVX_GLB float *out = reinterpret_cast<KVX_GLB float *>(a.part) + ((static_cast<uint64_t>(req) * a.splits + split) * queries + index) * kLatent + round * kJoinCols + c * 4;
-                        *reinterpret_cast<KVX_GLB f32x4 *>(out) = x;
-                    }
-                }
-            }
-            if (round + 1 < RW) __syncthreads();
-        }
-    } else {
-#pragma unroll
-        for (int w = 0; w < RW; ++w) {
-            if (query[w] >= queries) continue;
-            if (a.splits == 1) {
-                const float inv = sum[w] == 0.0f ? 0.0f : __builtin_amdgcn_rcpf(sum[w]);
-                KVX_GLB T *out = reinterpret_cast<KVX_GLB T *>(a.out) + (row0 + query[w]) * kLatent + grp * 4;
-#pragma unroll
-                for (int d = 0; d < kLatent / 16; ++d) {
-                    keep_in_acc(o[d][w]);
-                    *reinterpret_cast<KVX_GLB u32x2 *>(out + d * 16) =
-                        u32x2{pack2<T>(o[d][w][0] * inv, o[d][w][1] * inv), pack2<T>(o[d][w][2] * inv, o[d][w][3] * inv)};
-                }
-            } else {
-                KVX_GLB float *out = reinterpret_cast<KVX_GLB float *>(a.part) + ((static_cast<uint64_t>(req) * a.splits + split) * queries + query[w]) * kLatent + grp * 4;
-#pragma unroll
-                for (int d = 0; d < kLatent / 16; ++d) {
-                    keep_in_acc(o[d][w]);
-                    *reinterpret_cast<KVX_GLB f32x4 *>(out + d * 16) = o[d][w];
-                }
-            }
-        }
-    }
-    if (wk == 0 && grp == 0) {
-#pragma unroll
-        for (int w = 0; w < RW; ++w) {
-            if (query[w] >= queries) continue;
-            if (a.splits == 1) {
-                if (a.lse != 0) {
-                    reinterpret_cast<KVX_GLB float *>(a.lse)[row0 + query[w]] =
-                        sum[w] == 0.0f ? -INFINITY : (top[w] + __builtin_amdgcn_logf(sum[w])) * 0.6931471805599453f;
-                }
-            } else {
-                reinterpret_cast<KVX_GLB f32x2 *>(a.partStat)[(static_cast<uint64_t>(req) * a.splits + split) * queries + query[w]] = f32x2{top[w], sum[w]};
-            }
+    if (wave == 0 && grp == 0 && query < queries) {
+        if (a.splits > 1) {
+            reinterpret_cast<KVX_GLB f32x2 *>(a.partStat)[part0 + query] = f32x2{most, all};
+        } else if (a.lse != 0) {
+            reinterpret_cast<KVX_GLB float *>(a.lse)[row0 + query] =
+                all == 0.0f ? -INFINITY : (most + __builtin_amdgcn_logf(all)) * 0.6931471805599453f;
         }
     }
 }
@@ -622,33 +357,51 @@ __global__ __launch_bounds__(kThreads) void kvx_tree_attention_join(AttnArgs a)
 }
 
 template <int DTYPE, int QUANT>
-void launch(const AttnArgs &a, const AttnPlan &p, hipStream_t stream)
+void launch(const AttnArgs &a, hipStream_t stream)
 {
-    auto *kernel = p.rows == 16   ? kvx_tree_attention<DTYPE, QUANT, 1, 1>
-                   : p.rows == 32 ? kvx_tree_attention<DTYPE, QUANT, 2, 1>
-                   : p.rows == 64 ? kvx_tree_attention<DTYPE, QUANT, 2, 2>
-                                  : kvx_tree_attention<DTYPE, QUANT, 2, 4>;
     const uint32_t items = a.reqs * a.splits * a.queryTiles;
-    hipLaunchKernelGGL(kernel, dim3((items + 7u) / 8u * 8u), dim3(kThreads), 0, stream, a);
-    if (a.splits > 1) {
-        const uint64_t rows = static_cast<uint64_t>(a.reqs) * a.draft * a.heads;
-        hipLaunchKernelGGL(kvx_tree_attention_join<DTYPE>, dim3(static_cast<uint32_t>((rows + 3) / 4)), dim3(kThreads), 0,
-                           stream, a);
-    }
+    hipLaunchKernelGGL((kvx_tree_attention<DTYPE, QUANT>), dim3((items + 7u) / 8u * 8u), dim3(kThreads), 0, stream, a);
 }
 
 }  // namespace
 
-AttnPlan plan_tree_attention(uint32_t reqs, uint32_t draft, uint32_t heads, uint32_t topK, bool drafted)
+// Queries a workgroup and workgroups that share a query's keys, by the time that
+// each way is expected to take: a workgroup's start and end, its tiles one after
+// another (16 queries: four at a time), as many rounds of workgroups as the 256
+// CUs need, and the joining.  The figures are microseconds measured on an MI355X
+// with all CUs at work; what they decide, measured both ways (us):
+//   64 requests x 128 queries, 2048 keys: 16 wide 101, 64 in 2 splits 75, 128 in 4 splits 81
+//   4 x 4096 queries, 8192 keys: 16 wide 587, 64 wide 373, 128 in 2 splits 316
+//   1 x 256 queries, 2048 keys: 16 in 8 splits 21, 64 in 16 splits 29, 128 in 16 splits 39
+AttnPlan plan_tree_attention(uint32_t reqs, uint32_t draft, uint32_t heads, uint32_t topK, bool drafted, bool codes)
 {
-    AttnPlan p{};
+    struct Width {
+        uint32_t rows, atOnce;
+        float ends, tiles16, tiles8;     // of 16-bit and of 8-bit rows
+    };
+    constexpr Width widths[] = {{16, 4, 9.5f, 1.8f, 2.3f}, {64, 1, 12.0f, 1.42f, 1.85f}, {128, 1, 15.0f, 2.15f, 2.55f}};
     const uint32_t queries = draft * heads;
-    p.rows = queries <= 16 ? 16 : (queries <= 32 ? 32 : (queries <= 64 ? 64 : 128));
-    p.queryTiles = (queries + p.rows - 1) / p.rows;
-    const uint32_t tiles = (topK + (drafted ? draft : 0u) + kTile - 1) / kTile;
-    const uint32_t items = reqs * p.queryTiles;
-    const uint32_t groups = p.rows <= 32 ? 4 : (p.rows == 64 ? 2 : 1);
-    p.splits = std::max(1u, std::min(256u / std::max(items, 1u), tiles / (2 * groups)));
+    const uint32_t tiles = std::max(1u, (topK + (drafted ? draft : 0u) + kTile - 1) / kTile);
+    AttnPlan p{};
+    float best = 0.0f;
+    for (const Width &w : widths) {
+        const uint32_t queryTiles = (queries + w.rows - 1) / w.rows;
+        if (w.rows > 16 && queries <= w.rows / 4) break;       // (mostly empty)
+        for (uint32_t splits = 1; splits <= std::min(tiles, 64u); splits += splits < 4 ? 1 : splits / 2) {
+            const uint64_t items = static_cast<uint64_t>(reqs) * queryTiles * splits;
+            if (splits > 1 && items > 1024) break;
+            const uint32_t steps = ((tiles + splits - 1) / splits + w.atOnce - 1) / w.atOnce;
+            const float rounds = static_cast<float>((items + 255) / 256);
+            float us = (w.ends + steps * (codes ? w.tiles8 : w.tiles16)) * rounds;
+            if (splits > 1) us += 5.0f + static_cast<float>(reqs) * queries * splits * (kLatent * 4) * 0.3e-6f;
+            if (p.rows == 0 || us < best) {
+                best = us;
+                p.rows = w.rows;
+                p.queryTiles = queryTiles;
+                p.splits = splits;
+            }
+        }
+    }
     if (p.splits > 1) p.floats = static_cast<uint64_t>(reqs) * p.splits * queries * (kLatent + 2);
     return p;
 }
@@ -660,14 +413,24 @@ hipError_t launch_tree_attention(AttnArgs a, const AttnPlan &p, float *scratch, 
     a.splits = p.splits;
     a.part = reinterpret_cast<uint64_t>(scratch);
     a.partStat = a.part + static_cast<uint64_t>(a.reqs) * p.splits * a.draft * a.heads * kLatent * sizeof(float);
-    if (dtype == KVX_DTYPE_BF16) {
-        if (quant == KVX_QUANT_NONE) launch<KVX_DTYPE_BF16, KVX_QUANT_NONE>(a, p, stream);
-        else if (quant == KVX_QUANT_LATENT) launch<KVX_DTYPE_BF16, KVX_QUANT_LATENT>(a, p, stream);
-        else launch<KVX_DTYPE_BF16, KVX_QUANT_ROW>(a, p, stream);
+    if (p.rows >= 64) {
+        launch_tree_attention_wide(a, p, dtype, quant, stream);
+    } else if (dtype == KVX_DTYPE_BF16) {
+        if (quant == KVX_QUANT_NONE) launch<KVX_DTYPE_BF16, KVX_QUANT_NONE>(a, stream);
+        else if (quant == KVX_QUANT_LATENT) launch<KVX_DTYPE_BF16, KVX_QUANT_LATENT>(a, stream);
+        else launch<KVX_DTYPE_BF16, KVX_QUANT_ROW>(a, stream);
     } else {
-        if (quant == KVX_QUANT_NONE) launch<KVX_DTYPE_FP16, KVX_QUANT_NONE>(a, p, stream);
-        else if (quant == KVX_QUANT_LATENT) launch<KVX_DTYPE_FP16, KVX_QUANT_LATENT>(a, p, stream);
-        else launch<KVX_DTYPE_FP16, KVX_QUANT_ROW>(a, p, stream);
+        if (quant == KVX_QUANT_NONE) launch<KVX_DTYPE_FP16, KVX_QUANT_NONE>(a, stream);
+        else if (quant == KVX_QUANT_LATENT) launch<KVX_DTYPE_FP16, KVX_QUANT_LATENT>(a, stream);
+        else launch<KVX_DTYPE_FP16, KVX_QUANT_ROW>(a, stream);
+    }
+    if (a.splits > 1) {
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+        const uint64_t rows = static_cast<uint64_t>(a.reqs) * a.draft * a.heads;
+        const dim3 grid(static_cast<uint32_t>((rows + 3) / 4));
+        if (dtype == KVX_DTYPE_BF16) hipLaunchKernelGGL(kvx_tree_attention_join<KVX_DTYPE_BF16>, grid, dim3(256), 0, stream, a);
+        else hipLaunchKernelGGL(kvx_tree_attention_join<KVX_DTYPE_FP16>, grid, dim3(256), 0, stream, a);
     }
     return hipGetLastError();
 }

@@ -1,0 +1,234 @@
+// What the attention kernels share: the tile of keys in LDS, the matrix product
+// of a type, the reductions over the lanes of a query.
+#pragma once
+
+#include "row_format.h"
+
+namespace kvx {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kTile = 32;                 // keys a tile
+constexpr int kPanels = kDim / 64;        // a row in LDS: 9 panels of 64 values (128 bytes)
+constexpr int kPanelBytes = kTile * 128;
+constexpr int kTileBytes = kPanels * kPanelBytes;
+constexpr int kChunk = 64;                // tiles whose rows are looked up at a time
+constexpr int kSlots = kChunk * kTile / kThreads;
+constexpr float kRise = 8.0f;             // a maximum may rise by 2^8 before the output is scaled down again
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+#define KVX_LDS __attribute__((address_space(3)))
+#define KVX_GLB __attribute__((address_space(1)))
+
+// what a key without a row reads
+__device__ __align__(128) uint8_t kvx_no_row[kDim * 2];
+
+template <int DTYPE>
+struct Elem;
+template <>
+struct Elem<KVX_DTYPE_BF16> {
+    typedef __bf16 T;
+    static constexpr uint32_t special = 0x7F80u;   // exponent of infinities and NaN
+    static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c)
+    {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c,
+                                                       0, 0, 0);
+    }
+    static __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c)
+    {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c,
+                                                       0, 0, 0);
+    }
+    static __device__ __forceinline__ uint32_t from_codes(uint32_t codes, float scale, bool high)
+    {
+        return __builtin_bit_cast(uint32_t, high ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, true)
+                                                 : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, false));
+    }
+};
+template <>
+struct Elem<KVX_DTYPE_FP16> {
+    typedef _Float16 T;
+    static constexpr uint32_t special = 0x7C00u;
+    static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c)
+    {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0,
+                                                      0, 0);
+    }
+    static __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c)
+    {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0,
+                                                      0, 0);
+    }
+    static __device__ __forceinline__ uint32_t from_codes(uint32_t codes, float scale, bool high)
+    {
+        return __builtin_bit_cast(uint32_t, high ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, scale, true)
+                                                 : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, scale, false));
+    }
+};
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b)
+{
+    typedef T T2 __attribute__((ext_vector_type(2)));
+    T2 v;
+    v[0] = static_cast<T>(a);
+    v[1] = static_cast<T>(b);
+    return __builtin_bit_cast(uint32_t, v);
+}
+
+// Over the G lanes that hold scores of one query (lane % (64 / G)).
+template <int G, typename F>
+__device__ __forceinline__ float over_query(float x, F f)
+{
+    typedef unsigned int u2 __attribute__((ext_vector_type(2)));
+    u2 v = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = f(__uint_as_float(v[0]), __uint_as_float(v[1]));
+    if (G == 2) return x;
+    v = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return f(__uint_as_float(v[0]), __uint_as_float(v[1]));
+}
+
+// The output stays in the accumulation registers: without this the compiler
+// keeps second copies of it around each place that scales it, and spills.
+template <typename V>
+__device__ __forceinline__ void keep_in_acc(V &x) { asm volatile("" : "+a"(x)); }
+
+// Byte of the 16-byte chunk c (0..7) of row r in a panel: rows one after
+// another are 128 bytes apart, so the chunks of 8 rows are permuted to spread a
+// column over the banks.
+__device__ __forceinline__ uint32_t chunk_at(uint32_t r, uint32_t c) { return r * 128u + ((c ^ (r & 7u)) << 4); }
+
+// A drafted row that holds a NaN or an infinity must not reach the queries that
+// do not see it, whose weight 0 would turn it into a NaN; those that see it have
+// a score that is one already.  Such values become zeros in row r of the tile:
+// a wave a row, 16 bytes of its 512 columns a lane.
+template <int DTYPE>
+__device__ __forceinline__ void clean_row(uint32_t tile, uint32_t lane, uint32_t chunk)
+{
+    constexpr uint32_t special = Elem<DTYPE>::special;
+    KVX_LDS u32x4 *at = (KVX_LDS u32x4 *)(uintptr_t)(tile + (lane >> 3) * kPanelBytes + chunk);
+    u32x4 x = *at;
+    bool dirty = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const bool low = (x[i] & special) == special, high = (x[i] & (special << 16)) == special << 16;
+        x[i] &= (low ? 0xFFFF0000u : ~0u) & (high ? 0xFFFFu : ~0u);
+        dirty = dirty || low || high;
+    }
+    if (dirty) *at = x;
+}
+
+// 16 bytes a lane from memory at from + OFFSET to LDS at base + lane * 16, not
+// waited for: the caller counts the loads (wait_loads).  The instruction adds
+// its offset on both sides.
+template <int OFFSET>
+__device__ __forceinline__ void load_to_lds(const uint8_t *from, uint32_t base)
+{
+    // (a wait state between the write of m0 and its use)
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off offset:%2" ::"v"(from), "s"(base - OFFSET), "n"(OFFSET) : "memory");
+}
+
+// ... 4 bytes a lane, to base + lane * 4.
+__device__ __forceinline__ void load_to_lds4(const uint8_t *from, uint32_t base)
+{
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(from), "s"(base) : "memory");
+}
+
+// Panel p of a row, p known where this is unrolled.
+__device__ __forceinline__ void load_panel(const uint8_t *from, int p, uint32_t base)
+{
+    switch (p) {
+    case 0: return load_to_lds<0>(from, base);
+    case 1: return load_to_lds<128>(from, base);
+    case 2: return load_to_lds<256>(from, base);
+    case 3: return load_to_lds<384>(from, base);
+    case 4: return load_to_lds<512>(from, base);
+    case 5: return load_to_lds<640>(from, base);
+    case 6: return load_to_lds<768>(from, base);
+    case 7: return load_to_lds<896>(from, base);
+    default: return load_to_lds<1024>(from, base);
+    }
+}
+
+template <int LEFT>
+__device__ __forceinline__ void wait_loads()
+{
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LEFT) : "memory");
+}
+
+// All but the last n panels' loads (4 each), n known where this is unrolled.
+__device__ __forceinline__ void wait_panels(int n)
+{
+    switch (n) {
+    case 0: return wait_loads<0>();
+    case 1: return wait_loads<4>();
+    case 2: return wait_loads<8>();
+    case 3: return wait_loads<12>();
+    case 4: return wait_loads<16>();
+    case 5: return wait_loads<20>();
+    case 6: return wait_loads<24>();
+    case 7: return wait_loads<28>();
+    default: return wait_loads<32>();
+    }
+}
+
+// Every wave's LDS reads are done and what it waited for is there.
+__device__ __forceinline__ void meet() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// The part of a call that a workgroup takes.  Consecutive parts go to one XCD
+// (workgroups go to the 8 XCDs in turn), so that the workgroups that read the
+// same keys share its L2.
+struct AttnItem {
+    bool real;
+    uint32_t req, split, queryTile;
+    uint32_t keys;                       // of the request: selected and drafted
+    uint32_t tile0, tile1;               // of the range
+    __device__ __forceinline__ explicit AttnItem(const AttnArgs &a)
+    {
+        const uint32_t total = a.reqs * a.splits * a.queryTiles, each = (total + 7u) / 8u;
+        const uint32_t i = (blockIdx.x & 7u) * each + (blockIdx.x >> 3);
+        real = (blockIdx.x >> 3) < each && i < total;
+        queryTile = i % a.queryTiles;
+        split = i / a.queryTiles % a.splits;
+        req = i / a.queryTiles / a.splits;
+        keys = a.topK + (a.draftSlots != 0 ? a.draft : 0u);
+        const uint64_t tiles = (keys + kTile - 1) / kTile;
+        tile0 = static_cast<uint32_t>(tiles * split / a.splits);
+        tile1 = static_cast<uint32_t>(tiles * (split + 1) / a.splits);
+    }
+};
+
+// Slots of the chunk of tiles from c0 on, kThreads apart (-1 past the range).
+__device__ __forceinline__ void read_slots(const AttnArgs &a, const AttnItem &item, uint32_t c0, int32_t (&slot)[kSlots])
+{
+#pragma unroll
+    for (int n = 0; n < kSlots; ++n) {
+        const uint32_t k = c0 * kTile + n * kThreads + threadIdx.x;
+        slot[n] = -1;
+        if (k < min(item.keys, item.tile1 * kTile)) {
+            slot[n] = k < a.topK
+                          ? reinterpret_cast<const KVX_GLB int32_t *>(a.slots)[static_cast<uint64_t>(item.req) * a.topK + k]
+                          : reinterpret_cast<const KVX_GLB int32_t *>(a.draftSlots)[static_cast<uint64_t>(item.req) * a.draft + k - a.topK];
+        }
+    }
+}
+
+// ... into LDS, -1 where they name no row.
+__device__ __forceinline__ void look_up(const AttnArgs &a, const AttnItem &item, const int32_t (&slot)[kSlots], int32_t *rowOf)
+{
+#pragma unroll
+    for (int n = 0; n < kSlots; ++n) {
+        const bool is = hot_row(slot[n], item.req, a.reqStride, a.hotRows, a.overflowSlot) >= 0;
+        rowOf[n * kThreads + threadIdx.x] = is ? slot[n] : -1;
+    }
+}
+
+}  // namespace
+}  // namespace kvx

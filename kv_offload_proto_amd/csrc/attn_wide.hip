@@ -1,0 +1,474 @@
+// Attention over the hot buffer for requests of many queries (kvx/kvx_attn.h;
+// attn.hip has the few).
+//
+// Four waves take 16 or 32 queries each and share every tile of 32 keys, of
+// which each brings 8 rows to LDS.  A wave keeps its queries and the whole of
+// their output in registers, so one wave fills a SIMD and nothing else hides
+// its latencies: the work on a tile is cut in two and overlapped with that of
+// the next one,
+//
+//   scores of tile t + 1  (matrix)   with  loads, conversion of 8-bit rows
+//   output of tile t      (matrix)   with  maxima and weights of tile t + 1
+//
+// and the loads of a later tile are issued between the matrix products, one at
+// a time, because a load of 16 bytes a lane occupies the address unit for about
+// as long as a matrix product the matrix unit.
+//
+// Scores are held transposed, S^T = K Q^T (keys down, queries across the
+// lanes), so that a lane's scores, its running maximum and its sum all belong
+// to one query, and so that the weights are, as they come, the operand of
+// O^T = V^T P^T, where V is the first 512 columns of the same rows: a matrix
+// product takes its keys in any order, as long as both operands have the same.
+// With G groups of lanes (4 of 16 or 2 of 32 queries) a product gives lane l
+// the keys 4 G i + 4 (l / (64 / G)) + 0..3, i = 0, 1, ..
+//
+// The matrix unit and LDS bound it.  A tile's keys and values are read from LDS
+// once for every wave, 36 + 32 KB, for 32 queries while the matrix unit has
+// 2176 cycles of work on them and LDS (128 bytes a cycle) 2413 for the four
+// waves and the tile coming in; for 16 queries a wave twice that per product.
+#include "attn_tile.h"
+
+namespace kvx {
+namespace {
+
+// Byte of the 16-byte chunk c of row r in a panel: as chunk_at, and the upper 16
+// rows' chunks exchanged in pairs, because a read of 32 rows takes rows r and
+// r + 24 at once.
+__device__ __forceinline__ uint32_t chunk_in(uint32_t r, uint32_t c) { return chunk_at(r, c ^ (r >> 4)); }
+
+template <int LEFT>
+__device__ __forceinline__ void wait_loads_and_meet()
+{
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LEFT) : "memory");
+}
+
+// The matrix product of 64 / G queries: keys by 16 / 32 values each, or columns
+// by as many keys.
+template <int DTYPE, int G>
+struct Product;
+template <int DTYPE>
+struct Product<DTYPE, 4> {
+    typedef f32x4 Acc;
+    static __device__ __forceinline__ Acc mul(u32x4 a, u32x4 b, Acc c) { return Elem<DTYPE>::mfma(a, b, c); }
+};
+template <int DTYPE>
+struct Product<DTYPE, 2> {
+    typedef f32x16 Acc;
+    static __device__ __forceinline__ Acc mul(u32x4 a, u32x4 b, Acc c) { return Elem<DTYPE>::mfma32(a, b, c); }
+};
+
+template <int DTYPE, int QUANT, int G>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))) void kvx_tree_attention_wide(AttnArgs a)
+{
+    typedef Elem<DTYPE> E;
+    typedef typename E::T T;
+    typedef Product<DTYPE, G> P;
+    typedef typename P::Acc Acc;
+    using F = RowForm<QUANT>;
+    constexpr bool kCodes = QUANT != KVX_QUANT_NONE;
+    constexpr int kRows = 64 / G;                    // queries of a wave
+    constexpr int kAcc = kRows / G;                  // values of a product in a lane
+    constexpr int kSteps = kDim / (8 * G);           // products over a row's values
+    constexpr int kKeyTiles = kTile / kRows;         // ... and over a tile's keys: scores
+    constexpr int kKeySteps = kTile / (8 * G);       // ... output
+    constexpr int kScores = kKeyTiles * kAcc;        // of a lane and tile: 8 or 16
+    constexpr int kCols = kLatent / kRows;           // products over a row's columns
+    constexpr int kKeysAhead = 4 / kKeyTiles + 1, kColsAhead = 3 / kKeySteps + 1;   // operands read ahead
+    // Buffers of whole tiles: the two worked on, and for 16-bit rows the two
+    // under way; 8-bit rows arrive in buffers of their own and are converted
+    // into a third.
+    constexpr int kBuffers = kCodes ? 3 : 4;
+    constexpr int kRawPanels = 5;                    // 640 bytes of a row: codes, then the rotary part or scales
+    constexpr int kRawScales = F::raw != 0 ? 256 : 0;                // a wave's scale bytes where they lie behind these
+    constexpr int kRawBytes = kCodes ? kTile * kRawPanels * 128 + 4 * kRawScales : 0;
+    constexpr int kLoads = kCodes ? kRawPanels + (kRawScales != 0 ? 1 : 0) : kPanels;   // of a wave for a tile
+
+    __shared__ __align__(128) uint8_t tiles[kBuffers * kTileBytes + 2 * kRawBytes];
+    __shared__ int32_t rowOf[kChunk * kTile];        // hot row within the request of each key, -1: none
+
+    const uint32_t lane = threadIdx.x & 63u;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t col = lane % kRows, grp = lane / kRows;
+    const uint32_t queries = a.draft * a.heads;
+
+    const AttnItem item(a);
+    if (!item.real) return;
+    const uint32_t req = item.req;
+
+    int32_t firstSlots[kSlots];
+    read_slots(a, item, item.tile0, firstSlots);     // (before the queries: the rows' addresses wait for them)
+
+    const uint32_t query = (item.queryTile * 4 + wave) * kRows + col;            // this lane's
+    u32x4 q[kSteps];
+    uint64_t sees;                                   // drafted tokens that the query sees
+    {
+        const uint32_t real = min(query, queries - 1);               // (what lies past the last query is not stored)
+        const uint32_t node = real / a.heads, head = real % a.heads;
+        const uint64_t at = a.q + req * a.qStrideB + node * a.qStrideT + head * a.qStrideH + grp * 16;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) q[s] = *reinterpret_cast<const KVX_GLB u32x4 *>(at + s * G * 16);
+        sees = a.treeMask != 0 ? reinterpret_cast<const KVX_GLB uint64_t *>(a.treeMask)[req * a.draft + node]
+                               : ~0ull >> (63u - node);
+    }
+    look_up(a, item, firstSlots, rowOf);
+    const uint32_t flip = a.negate ? 0x80008000u : 0u;               // a negative scale: negative queries
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) q[s] ^= flip;
+    float top = -INFINITY, sum = 0.0f;
+    Acc o[kCols];
+#pragma unroll
+    for (int d = 0; d < kCols; ++d) o[d] = Acc{};
+
+    const uint8_t *hot = reinterpret_cast<const uint8_t *>(a.hot) + req * a.reqStride * F::bytes;
+    const uint32_t ldsTiles = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((KVX_LDS uint8_t *)tiles));
+    const uint32_t ldsRaw = ldsTiles + kBuffers * kTileBytes;
+    // this lane's bytes of a tile: its key's chunk for a score step (8 / G steps
+    // a panel), and four columns of four keys for an output step
+    uint32_t atKey[kKeyTiles][8 / G], atValue[2][G];                 // ([1]: of the upper 16 keys)
+#pragma unroll
+    for (int h = 0; h < kKeyTiles; ++h) {
+#pragma unroll
+        for (int n = 0; n < 8 / G; ++n) atKey[h][n] = chunk_in(h * kRows + col, n * G + grp);
+    }
+#pragma unroll
+    for (int n = 0; n < G; ++n) {
+        // columns 16 * sixteen and on; with two groups the upper 16 lanes take those 32 columns on, not the next ones,
+        // which lie in the banks of the lower lanes' third and fourth key
+        const uint32_t sixteen = G == 4 ? n : n + ((lane >> 3) & 2u);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            atValue[h][n] = chunk_in(h * 16 + grp * 4 + ((lane >> 2) & 3u), sixteen * 2 + ((lane >> 1) & 1u)) + (lane & 1u) * 8u;
+        }
+    }
+
+    // ---- bringing a tile in: each wave 8 rows, 128 bytes of each a load ----
+    // (a tile past the chunk: rows of zeros, so that the count of the loads under way stays what it is)
+    auto rowStart = [&](uint32_t t, uint32_t n, uint32_t r) {
+        const int32_t row = rowOf[min(t, n - 1) * kTile + wave * 8 + r];
+        return row < 0 || t >= n ? kvx_no_row : hot + static_cast<uint64_t>(static_cast<uint32_t>(row)) * F::bytes;
+    };
+    struct Source {
+        const uint8_t *rows, *scales;
+        uint32_t to;
+    };
+    auto source = [&](uint32_t t, uint32_t n, uint32_t buffer) {
+        Source x;
+        x.rows = rowStart(t, n, lane >> 3) + (kCodes ? lane & 7u : (lane & 7u) ^ (lane >> 3) ^ (wave >> 1)) * 16;
+        x.scales = kRawScales != 0 ? rowStart(t, n, (lane >> 2) & 7u) + F::scaleAt + (lane & 3u) * 4 : nullptr;
+        x.to = kCodes ? ldsRaw + (t & 1u) * kRawBytes : ldsTiles + buffer;
+        return x;
+    };
+    auto loadPart = [&](const Source &x, int p) {
+        if (p >= kLoads) return;
+        if (kCodes && p == kRawPanels) load_to_lds4(x.scales, x.to + kTile * kRawPanels * 128 + wave * 256);
+        else load_panel(x.rows, p, x.to + p * kPanelBytes + wave * 1024);
+    };
+    // 8-bit rows: a wave converts the rows that it brought in, a panel of 128 codes at a time
+    u32x4 codes;
+    uint32_t fourScales;
+    auto readCodes = [&](uint32_t t, int p) {
+        const uint32_t raw = ldsRaw + (t & 1u) * kRawBytes;
+        codes = *(const KVX_LDS u32x4 *)(uintptr_t)(raw + (p * 4 + wave) * 1024 + lane * 16);
+        const uint32_t at = kRawScales != 0 ? raw + kTile * kRawPanels * 128 + wave * 256 + (lane >> 3) * 16 + p * 4
+                                            : raw + (4 * 4 + wave) * 1024 + (lane >> 3) * 128 + 64 + p * 4;
+        if (F::raw == 0 || p < 4) fourScales = *(const KVX_LDS uint32_t *)(uintptr_t)at;
+    };
+    auto writeValues = [&](uint32_t buffer, int p) {
+        const uint32_t r = wave * 8 + (lane >> 3), j = lane & 7u;
+        const uint32_t to = ldsTiles + buffer + p * 2 * kPanelBytes;
+        if (F::raw != 0 && p == 4) {
+            *(KVX_LDS u32x4 *)(uintptr_t)(to + chunk_in(r, j)) = codes;
+            return;
+        }
+        const float scale = __uint_as_float(((fourScales >> ((j >> 1) * 8)) & 255u) << 23);
+        u32x4 x, y;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            x[2 * i] = E::from_codes(codes[i], scale, false);
+            x[2 * i + 1] = E::from_codes(codes[i], scale, true);
+            y[2 * i] = E::from_codes(codes[2 + i], scale, false);
+            y[2 * i + 1] = E::from_codes(codes[2 + i], scale, true);
+        }
+        if (p < 4 || j < 4) {                        // (the fifth panel is half a panel of codes)
+            const uint32_t panel = to + (j >> 2) * kPanelBytes;
+            *(KVX_LDS u32x4 *)(uintptr_t)(panel + chunk_in(r, (j & 3u) * 2)) = x;
+            *(KVX_LDS u32x4 *)(uintptr_t)(panel + chunk_in(r, (j & 3u) * 2 + 1)) = y;
+        }
+    };
+
+    // ---- scores ----
+    Acc s[kKeyTiles];
+    u32x4 key[kKeysAhead + 1][kKeyTiles];
+    auto readKeys = [&](const KVX_LDS uint8_t *tile, int n) {
+#pragma unroll
+        for (int h = 0; h < kKeyTiles; ++h) {
+            key[n % (kKeysAhead + 1)][h] =
+                *reinterpret_cast<const KVX_LDS u32x4 *>(tile + atKey[h][n % (8 / G)] + n * G / 8 * kPanelBytes);
+        }
+    };
+    auto score = [&](int n) {
+#pragma unroll
+        for (int h = 0; h < kKeyTiles; ++h) s[h] = P::mul(key[n % (kKeysAhead + 1)][h], q[n], n == 0 ? Acc{} : s[h]);
+    };
+    float c[kScores], most;
+    // the scores of a tile, -infinity where the query does not see the key
+    auto takeScores = [&](uint32_t live, uint32_t k0, bool drafted) {
+#pragma unroll
+        for (int e = 0; e < kScores; ++e) c[e] = s[e / kAcc][e % kAcc];
+        if (live == ~0u && !drafted) return;
+        const uint32_t selected = k0 >= a.topK ? 0u : (a.topK - k0 >= 32u ? ~0u : (1u << (a.topK - k0)) - 1u);
+        uint32_t own = 0;                            // drafted tokens' bits of this tile
+        if (drafted) own = static_cast<uint32_t>(k0 >= a.topK ? sees >> (k0 - a.topK) : sees << min(a.topK - k0, 63u));
+        const uint32_t seen = (live & (selected | (own & ~selected))) >> (grp * 4);
+#pragma unroll
+        for (int e = 0; e < kScores; ++e) c[e] = (seen & (1u << (e / 4 * 4 * G + e % 4))) != 0 ? c[e] : -INFINITY;
+    };
+    auto lanesMost = [&](int part) {                 // (a NaN is left out; its weight is one)
+#pragma unroll
+        for (int e = part * 8; e < part * 8 + 8; ++e) most = e == 0 ? c[0] : fmaxf(most, c[e]);
+    };
+    // The weights are exp2(score - top) for a top at most 2^8 below the largest
+    // score so far: top moves, and the output is scaled, only when one rose by
+    // more.  The weights of a tile are made while the output before it is still
+    // being summed, so that is scaled (settle) when both are done.
+    float newTop, base, add;
+    bool rise;
+    auto decide = [&] {
+        most = over_query<G>(most, [](float x, float y) { return fmaxf(x, y); }) * a.scaleLog2;
+        rise = __any(most > top + kRise) != 0;
+        newTop = rise ? fmaxf(top, most) : top;
+        base = newTop == -INFINITY ? 0.0f : newTop;
+        add = 0.0f;
+    };
+    u32x4 weight[kKeySteps], newWeight[kKeySteps];
+    auto weigh = [&](int e) {
+        c[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(c[e], a.scaleLog2, -base));
+        add += c[e];
+        if (e & 1) newWeight[e / 8][e % 8 >> 1] = pack2<T>(c[e - 1], c[e]);
+    };
+    auto settle = [&] {
+        if (rise) {
+            const bool any = top != -INFINITY;       // (nothing is there to scale at the first tile)
+            const float keep = newTop == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top - newTop);
+            top = newTop;
+            if (__any(any)) {
+                sum *= keep;
+#pragma unroll
+                for (int d = 0; d < kCols; ++d) {
+                    keep_in_acc(o[d]);
+                    o[d] *= keep;
+                    keep_in_acc(o[d]);
+                }
+            }
+        }
+        sum += add;
+#pragma unroll
+        for (int n = 0; n < kKeySteps; ++n) weight[n] = newWeight[n];
+    };
+    u32x4 value[kColsAhead + 1][kKeySteps];
+    auto readColumns = [&](const KVX_LDS uint8_t *tile, int d) {
+#pragma unroll
+        for (int n = 0; n < kKeySteps; ++n) {
+            // keys 8 G n + 0.. and 8 G n + 4 G + 0..
+            auto at = [&](int k) { return (KVX_LDS s16x4 *)(tile + atValue[k / 16][d % G] + d / G * kPanelBytes + k % 16 * 128); };
+            const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at(8 * G * n));
+            const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at(8 * G * n + 4 * G));
+            value[d % (kColsAhead + 1)][n] = __builtin_bit_cast(u32x4, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+        }
+    };
+
+    for (uint32_t c0 = item.tile0; c0 < item.tile1; c0 += kChunk) {
+        const uint32_t n = min(static_cast<uint32_t>(kChunk), item.tile1 - c0);
+        if (c0 != item.tile0) {
+            int32_t slots[kSlots];
+            read_slots(a, item, c0, slots);
+            wait_loads_and_meet<0>();                // (the chunk before has been read, and its last loads have landed)
+            look_up(a, item, slots, rowOf);
+        }
+        __syncthreads();
+        auto liveKeys = [&](uint32_t t) { return static_cast<uint32_t>(__ballot(rowOf[t * kTile + (lane & 31u)] >= 0)); };
+        auto isDrafted = [&](uint32_t t) { return (c0 + t + 1) * kTile > a.topK && a.draftSlots != 0; };
+
+        // the first tile's scores
+        if constexpr (kCodes) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const Source x = source(t, n, 0);
+#pragma unroll
+                for (int p = 0; p < kLoads; ++p) loadPart(x, p);
+            }
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                wait_loads<kLoads>();                // tiles 0 and 1; one other is under way
+#pragma unroll
+                for (int p = 0; p < kRawPanels; ++p) {
+                    readCodes(t, p);
+                    writeValues(t * kTileBytes, p);
+                }
+                const Source x = source(t + 2, n, 0);
+#pragma unroll
+                for (int p = 0; p < kLoads; ++p) loadPart(x, p);
+            }
+            meet();
+        } else {
+#pragma unroll
+            for (int t = 0; t < 3; ++t) {
+                const Source x = source(t, n, t * kTileBytes);
+#pragma unroll
+                for (int p = 0; p < kLoads; ++p) loadPart(x, p);
+            }
+            wait_loads_and_meet<2 * kLoads>();
+        }
+        {
+            const KVX_LDS uint8_t *tile = (KVX_LDS uint8_t *)(uintptr_t)ldsTiles;
+            const uint32_t live = liveKeys(0);
+#pragma unroll
+            for (int i = 0; i < kKeysAhead; ++i) readKeys(tile, i);
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+                if (i + kKeysAhead < kSteps) readKeys(tile, i + kKeysAhead);
+                score(i);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            takeScores(live, c0 * kTile, isDrafted(0));
+#pragma unroll
+            for (int i = 0; i < kScores / 8; ++i) lanesMost(i);
+            decide();
+#pragma unroll
+            for (int e = 0; e < kScores; ++e) weigh(e);
+            settle();
+        }
+
+        uint32_t buffer = 0;                         // of tile t
+        auto ahead = [&](uint32_t by) {
+            const uint32_t b = buffer + by * kTileBytes;
+            return b >= kBuffers * kTileBytes ? b - kBuffers * kTileBytes : b;
+        };
+        Source from = source(3, n, ahead(3));        // of tile t + 3 (16-bit rows)
+        uint32_t live = liveKeys(min(1u, n - 1));    // of tile t + 1
+        for (uint32_t t = 0; t < n; ++t) {
+            // tile t + 1 has landed (16-bit rows) or been converted, and tile t - 1 has been read
+            if constexpr (kCodes) meet();
+            else wait_loads_and_meet<kLoads>();
+            const KVX_LDS uint8_t *tile = (KVX_LDS uint8_t *)(uintptr_t)(ldsTiles + buffer);
+            const KVX_LDS uint8_t *nextTile = (KVX_LDS uint8_t *)(uintptr_t)(ldsTiles + ahead(1));
+            const bool more = t + 1 < n;
+            if (isDrafted(t)) {
+                const uint32_t k0 = (c0 + t) * kTile, last = min(item.keys - k0, static_cast<uint32_t>(kTile));
+                for (uint32_t r = (k0 >= a.topK ? 0u : a.topK - k0) + wave; r < last; r += 4) {
+                    clean_row<DTYPE>(ldsTiles + buffer, lane, chunk_in(r, lane & 7u));
+                }
+                meet();
+            }
+            if (kCodes) wait_loads<kLoads>();        // tile t + 2
+            if (more) {
+#pragma unroll
+                for (int i = 0; i < kKeysAhead; ++i) readKeys(nextTile, i);
+#pragma unroll
+                for (int i = 0; i < kSteps; ++i) {
+                    if (i + kKeysAhead < kSteps) readKeys(nextTile, i + kKeysAhead);
+                    if (i + kColsAhead >= kSteps) readColumns(tile, i + kColsAhead - kSteps);
+                    if (i % (kSteps / 18) == 0) {    // (eighteenths of the way)
+                        const int part = i / (kSteps / 18);
+                        if (!kCodes && part % 2 == 0) loadPart(from, part / 2);
+                        if (kCodes && part % 3 == 0 && part / 3 < kRawPanels) readCodes(t, part / 3);
+                        if (kCodes && part % 3 == 2 && part / 3 < kRawPanels) writeValues(ahead(2), part / 3);
+                        if (kCodes && part == 16) from = source(t + 4, n, 0);
+                    }
+                    score(i);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                takeScores(live, (c0 + t + 1) * kTile, isDrafted(t + 1));
+            } else {
+#pragma unroll
+                for (int i = 0; i < kColsAhead; ++i) readColumns(tile, i);
+#pragma unroll
+                for (int p = 0; p < kLoads; ++p) {
+                    if (!kCodes) loadPart(from, p);
+                }
+            }
+#pragma unroll
+            for (int d = 0; d < kCols; ++d) {
+                if (d + kColsAhead < kCols) readColumns(tile, d + kColsAhead);
+                constexpr int kPart = kCols / 16;    // (sixteenths of the way)
+                if (d % kPart == 0) {
+                    const int part = d / kPart;
+                    if (part < kScores / 8) lanesMost(part);
+                    if (part == 2) decide();
+#pragma unroll
+                    for (int e = (part - 3) * kScores / 12; part >= 3 && part < 15 && e < (part - 2) * kScores / 12; ++e) weigh(e);
+                    if (kCodes && part >= 8) loadPart(from, part - 8);
+                    // what the next round begins with
+                    if (part == 3) live = liveKeys(min(t + 2, n - 1));
+                    if (!kCodes && part == 5) from = source(t + 4, n, buffer);
+                }
+#pragma unroll
+                for (int i = 0; i < kKeySteps; ++i) o[d] = P::mul(value[d % (kColsAhead + 1)][i], weight[i], o[d]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if (more) settle();
+            buffer = ahead(1);
+        }
+    }
+    wait_loads<0>();                                 // (nothing may land in LDS that is another workgroup's by then)
+
+    // of the i-th value of the d-th product, before the lane's group's four
+    auto column = [](int d, int i) { return G == 4 ? d * 16 : d / 2 * 64 + d % 2 * 16 + i / 8 * 32 + i / 4 % 2 * 8; };
+    const uint64_t row0 = static_cast<uint64_t>(req) * queries;        // first output row of the request
+    sum = over_query<G>(sum, [](float x, float y) { return x + y; });
+    if (query >= queries) return;
+    if (a.splits == 1) {
+        const float inv = sum == 0.0f ? 0.0f : __builtin_amdgcn_rcpf(sum);
+        KVX_GLB T *out = reinterpret_cast<KVX_GLB T *>(a.out) + (row0 + query) * kLatent + grp * 4;
+#pragma unroll
+        for (int d = 0; d < kCols; ++d) {
+            keep_in_acc(o[d]);
+#pragma unroll
+            for (int i = 0; i < kAcc; i += 4) {
+                *reinterpret_cast<KVX_GLB u32x2 *>(out + column(d, i)) =
+                    u32x2{pack2<T>(o[d][i] * inv, o[d][i + 1] * inv), pack2<T>(o[d][i + 2] * inv, o[d][i + 3] * inv)};
+            }
+        }
+        if (a.lse != 0 && grp == 0) {
+            reinterpret_cast<KVX_GLB float *>(a.lse)[row0 + query] =
+                sum == 0.0f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * 0.6931471805599453f;
+        }
+    } else {
+        const uint64_t at = (static_cast<uint64_t>(req) * a.splits + item.split) * queries + query;
+        KVX_GLB float *out = reinterpret_cast<KVX_GLB float *>(a.part) + at * kLatent + grp * 4;
+#pragma unroll
+        for (int d = 0; d < kCols; ++d) {
+            keep_in_acc(o[d]);
+#pragma unroll
+            for (int i = 0; i < kAcc; i += 4) {
+                *reinterpret_cast<KVX_GLB f32x4 *>(out + column(d, i)) = f32x4{o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]};
+            }
+        }
+        if (grp == 0) reinterpret_cast<KVX_GLB f32x2 *>(a.partStat)[at] = f32x2{top, sum};
+    }
+}
+
+template <int DTYPE, int QUANT>
+void launch(const AttnArgs &a, const AttnPlan &p, hipStream_t stream)
+{
+    auto *kernel = p.rows == 64 ? kvx_tree_attention_wide<DTYPE, QUANT, 4> : kvx_tree_attention_wide<DTYPE, QUANT, 2>;
+    const uint32_t items = a.reqs * a.splits * a.queryTiles;
+    hipLaunchKernelGGL(kernel, dim3((items + 7u) / 8u * 8u), dim3(kThreads), 0, stream, a);
+}
+
+}  // namespace
+
+void launch_tree_attention_wide(const AttnArgs &a, const AttnPlan &p, uint32_t dtype, uint32_t quant, hipStream_t stream)
+{
+    if (dtype == KVX_DTYPE_BF16) {
+        if (quant == KVX_QUANT_NONE) launch<KVX_DTYPE_BF16, KVX_QUANT_NONE>(a, p, stream);
+        else if (quant == KVX_QUANT_LATENT) launch<KVX_DTYPE_BF16, KVX_QUANT_LATENT>(a, p, stream);
+        else launch<KVX_DTYPE_BF16, KVX_QUANT_ROW>(a, p, stream);
+    } else {
+        if (quant == KVX_QUANT_NONE) launch<KVX_DTYPE_FP16, KVX_QUANT_NONE>(a, p, stream);
+        else if (quant == KVX_QUANT_LATENT) launch<KVX_DTYPE_FP16, KVX_QUANT_LATENT>(a, p, stream);
+        else launch<KVX_DTYPE_FP16, KVX_QUANT_ROW>(a, p, stream);
+    }
+}
+
+}  // namespace kvx

@@ -1242,7 +1242,8 @@ int kvx_tree_attention(uint64_t q, uint64_t q_stride_b, uint64_t q_stride_t, uin
         if (static_cast<uint64_t>(num_reqs) * draft * heads >= 1ull << 31) {
             throw Error("tree_attention: num_reqs * draft * heads must be below 2^31");
         }
-        const kvx::AttnPlan p = kvx::plan_tree_attention(num_reqs, draft, heads, top_k, draft_slots != 0);
+        const kvx::AttnPlan p = kvx::plan_tree_attention(num_reqs, draft, heads, top_k, draft_slots != 0,
+                                                          quant != KVX_QUANT_NONE);
         float *scratch = nullptr;
         std::unique_lock<std::mutex> lk(g_scratchMu, std::defer_lock);
         if (p.floats != 0) {

@@ -78,12 +78,15 @@ struct AttnArgs {
 
 // How a call is cut up.
 struct AttnPlan {
-    uint32_t rows;          // queries a workgroup: 16, 32, 64 or 128
+    uint32_t rows;          // queries a workgroup: 16, 64 or 128
     uint32_t queryTiles;    // ... and how many of these a request has
     uint32_t splits;        // workgroups that share a query's keys
     uint64_t floats;        // scratch for their outputs
 };
-AttnPlan plan_tree_attention(uint32_t reqs, uint32_t draft, uint32_t heads, uint32_t topK, bool drafted);
+AttnPlan plan_tree_attention(uint32_t reqs, uint32_t draft, uint32_t heads, uint32_t topK, bool drafted,
+                             bool codes);
+void launch_tree_attention_wide(const AttnArgs &a, const AttnPlan &p, uint32_t dtype, uint32_t quant,
+                                hipStream_t stream);   // 64 and 128 queries a workgroup
 hipError_t launch_tree_attention(AttnArgs a, const AttnPlan &p, float *scratch, uint32_t dtype, uint32_t quant,
                                  hipStream_t stream);
 

@@ -215,9 +215,9 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
 #pragma unroll
             for (int j = 1; j < 8; ++j) most = fmaxf(most, s[j >> 2][j & 3]);
             most = over_query<4>(most, [](float x, float y) { return fmaxf(x, y); }) * a.scaleLog2;
-            // The weights are exp2(score - top) for a top at most 2^8 below the
+            // The weights are exp2(score - top) for a top a little below the
             // largest score so far: the output is scaled only when one rose by more.
-            if (__any(most > top + kRise)) {
+            if (__any(most > top + E::rise)) {
                 const float now = fmaxf(top, most);
                 const bool any = top != -INFINITY;   // (nothing is there to scale at the first tile)
                 const float keep = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top - now);

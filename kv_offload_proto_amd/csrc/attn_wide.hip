@@ -227,7 +227,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
 #pragma unroll
         for (int e = part * 8; e < part * 8 + 8; ++e) most = e == 0 ? c[0] : fmaxf(most, c[e]);
     };
-    // The weights are exp2(score - top) for a top at most 2^8 below the largest
+    // The weights are exp2(score - top) for a top a little below the largest
     // score so far: top moves, and the output is scaled, only when one rose by
     // more.  The weights of a tile are made while the output before it is still
     // being summed, so that is scaled (settle) when both are done.
@@ -235,7 +235,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
     bool rise;
     auto decide = [&] {
         most = over_query<G>(most, [](float x, float y) { return fmaxf(x, y); }) * a.scaleLog2;
-        rise = __any(most > top + kRise) != 0;
+        rise = __any(most > top + E::rise) != 0;
         newTop = rise ? fmaxf(top, most) : top;
         base = newTop == -INFINITY ? 0.0f : newTop;
         add = 0.0f;

@@ -51,8 +51,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
     if (!item.real) return;
     const uint32_t req = item.req;
 
-    int32_t firstSlots[kSlots];
-    read_slots(a, item, item.tile0, firstSlots);     // (before the queries: the rows' addresses wait for them)
+    // (before the queries: the rows' addresses wait for them)
+    look_up(a, item, item.tile0, min(static_cast<uint32_t>(kChunk), item.tile1 - item.tile0), rowOf);
 
     const uint32_t query = item.queryTile * kRows + col;             // this lane's
     u32x4 q[kDim / 32];
@@ -66,7 +66,6 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
         sees = a.treeMask != 0 ? reinterpret_cast<const KVX_GLB uint64_t *>(a.treeMask)[req * a.draft + node]
                                : ~0ull >> (63u - node);
     }
-    look_up(a, item, firstSlots, rowOf);
     const uint32_t flip = a.negate ? 0x80008000u : 0u;               // a negative scale: negative queries
 #pragma unroll
     for (int s = 0; s < kDim / 32; ++s) q[s] ^= flip;
@@ -150,10 +149,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
     for (uint32_t c0 = item.tile0; c0 < item.tile1; c0 += kChunk) {
         const uint32_t chunk = min(static_cast<uint32_t>(kChunk), item.tile1 - c0);
         if (c0 != item.tile0) {
-            int32_t slots[kSlots];
-            read_slots(a, item, c0, slots);
             __syncthreads();
-            look_up(a, item, slots, rowOf);
+            look_up(a, item, c0, chunk, rowOf);
         }
         __syncthreads();
         if (wave < chunk) {
@@ -296,7 +293,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
     __syncthreads();
     const uint64_t row0 = static_cast<uint64_t>(req) * queries;      // first output row of the request
     const uint64_t part0 = (static_cast<uint64_t>(req) * a.splits + item.split) * queries;
-#pragma unroll
+#pragma unroll 2
     for (int n = 0; n < kRows * (kLatent / 4) / kThreads; ++n) {
         const uint32_t i = threadIdx.x + n * kThreads, c = i % (kLatent / 4), r = i / (kLatent / 4);
         f32x4 x = {};

@@ -13,7 +13,6 @@ constexpr int kPanels = kDim / 64;        // a row in LDS: 9 panels of 64 values
 constexpr int kPanelBytes = kTile * 128;
 constexpr int kTileBytes = kPanels * kPanelBytes;
 constexpr int kChunk = 64;                // tiles whose rows are looked up at a time
-constexpr int kSlots = kChunk * kTile / kThreads;
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -194,6 +193,7 @@ struct AttnItem {
     uint32_t req, split, queryTile;
     uint32_t keys;                       // of the request: selected and drafted
     uint32_t tile0, tile1;               // of the range
+    uint32_t slots;                      // of the request that lie in the buffer
     __device__ __forceinline__ explicit AttnItem(const AttnArgs &a)
     {
         const uint32_t total = a.reqs * a.splits * a.queryTiles, each = (total + 7u) / 8u;
@@ -206,32 +206,37 @@ struct AttnItem {
         const uint64_t tiles = (keys + kTile - 1) / kTile;
         tile0 = static_cast<uint32_t>(tiles * split / a.splits);
         tile1 = static_cast<uint32_t>(tiles * (split + 1) / a.splits);
+        const uint64_t base = req * a.reqStride;
+        slots = base >= a.hotRows ? 0u : static_cast<uint32_t>(min(a.hotRows - base, static_cast<uint64_t>(1u << 31)));
     }
 };
 
-// Slots of the chunk of tiles from c0 on, kThreads apart (-1 past the range).
-__device__ __forceinline__ void read_slots(const AttnArgs &a, const AttnItem &item, uint32_t c0, int32_t (&slot)[kSlots])
+// The slots of n tiles from c0 on into LDS, -1 where they name no row.  Four at
+// a time, and no more code than that: what a launch runs once it waits for,
+// about a microsecond for each 2 KB of instructions.
+__device__ __forceinline__ void look_up(const AttnArgs &a, const AttnItem &item, uint32_t c0, uint32_t n, int32_t *rowOf)
 {
+    const KVX_GLB int32_t *selected = reinterpret_cast<const KVX_GLB int32_t *>(a.slots) + static_cast<uint64_t>(item.req) * a.topK;
+    const KVX_GLB int32_t *drafted = reinterpret_cast<const KVX_GLB int32_t *>(a.draftSlots) + static_cast<uint64_t>(item.req) * a.draft;
+    constexpr uint32_t kBatch = 4;
+    bool past = false;
+#pragma unroll 1
+    for (uint32_t i = threadIdx.x; i < n * kTile; i += kBatch * kThreads) {
+        int32_t slot[kBatch];
 #pragma unroll
-    for (int n = 0; n < kSlots; ++n) {
-        const uint32_t k = c0 * kTile + n * kThreads + threadIdx.x;
-        slot[n] = -1;
-        if (k < min(item.keys, item.tile1 * kTile)) {
-            slot[n] = k < a.topK
-                          ? reinterpret_cast<const KVX_GLB int32_t *>(a.slots)[static_cast<uint64_t>(item.req) * a.topK + k]
-                          : reinterpret_cast<const KVX_GLB int32_t *>(a.draftSlots)[static_cast<uint64_t>(item.req) * a.draft + k - a.topK];
+        for (uint32_t j = 0; j < kBatch; ++j) {
+            const uint32_t k = c0 * kTile + i + j * kThreads;
+            slot[j] = -1;
+            if (i + j * kThreads < n * kTile && k < item.keys) slot[j] = k < a.topK ? selected[k] : drafted[k - a.topK];
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < kBatch; ++j) {
+            const bool is = static_cast<uint32_t>(slot[j]) < item.slots;
+            past = past || (slot[j] >= 0 && !is);
+            if (i + j * kThreads < kChunk * kTile) rowOf[i + j * kThreads] = is ? slot[j] : -1;
         }
     }
-}
-
-// ... into LDS, -1 where they name no row.
-__device__ __forceinline__ void look_up(const AttnArgs &a, const AttnItem &item, const int32_t (&slot)[kSlots], int32_t *rowOf)
-{
-#pragma unroll
-    for (int n = 0; n < kSlots; ++n) {
-        const bool is = hot_row(slot[n], item.req, a.reqStride, a.hotRows, a.overflowSlot) >= 0;
-        rowOf[n * kThreads + threadIdx.x] = is ? slot[n] : -1;
-    }
+    if (past) report_row(a.overflowSlot);
 }
 
 }  // namespace

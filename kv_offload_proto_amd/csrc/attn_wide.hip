@@ -95,8 +95,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
     if (!item.real) return;
     const uint32_t req = item.req;
 
-    int32_t firstSlots[kSlots];
-    read_slots(a, item, item.tile0, firstSlots);     // (before the queries: the rows' addresses wait for them)
+    // (before the queries: the rows' addresses wait for them)
+    look_up(a, item, item.tile0, min(static_cast<uint32_t>(kChunk), item.tile1 - item.tile0), rowOf);
 
     const uint32_t query = (item.queryTile * 4 + wave) * kRows + col;            // this lane's
     u32x4 q[kSteps];
@@ -110,7 +110,6 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
         sees = a.treeMask != 0 ? reinterpret_cast<const KVX_GLB uint64_t *>(a.treeMask)[req * a.draft + node]
                                : ~0ull >> (63u - node);
     }
-    look_up(a, item, firstSlots, rowOf);
     const uint32_t flip = a.negate ? 0x80008000u : 0u;               // a negative scale: negative queries
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) q[s] ^= flip;
@@ -280,10 +279,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
     for (uint32_t c0 = item.tile0; c0 < item.tile1; c0 += kChunk) {
         const uint32_t n = min(static_cast<uint32_t>(kChunk), item.tile1 - c0);
         if (c0 != item.tile0) {
-            int32_t slots[kSlots];
-            read_slots(a, item, c0, slots);
             wait_loads_and_meet<0>();                // (the chunk before has been read, and its last loads have landed)
-            look_up(a, item, slots, rowOf);
+            look_up(a, item, c0, n, rowOf);
         }
         __syncthreads();
         auto liveKeys = [&](uint32_t t) { return static_cast<uint32_t>(__ballot(rowOf[t * kTile + (lane & 31u)] >= 0)); };

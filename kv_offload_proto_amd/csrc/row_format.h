@@ -24,22 +24,27 @@ struct RowForm {
     static constexpr int bytes = (scaleAt + scales + 127) / 128 * 128;
 };
 
+// A slot named a row past the buffer: told in the tail-slot word.
+__device__ __forceinline__ void report_row(uint64_t overflowSlot)
+{
+    if (overflowSlot == 0) return;
+    // (the global address space: a flat access would have later LDS reads waited for in full)
+    typedef __attribute__((address_space(1))) unsigned long long Word;
+    unsigned long long none = 0;
+    __hip_atomic_compare_exchange_strong(reinterpret_cast<Word *>(overflowSlot), &none,
+                                         static_cast<unsigned long long>(KVX_OVERFLOW_ROW), __ATOMIC_RELAXED,
+                                         __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
 // Hot row of slot s of request b: -1 where there is none.  A row past the
-// buffer is none either, and told in the tail-slot word.
+// buffer is none either, and told.
 __device__ __forceinline__ int64_t hot_row(int32_t slot, uint64_t b, uint64_t reqStride, uint64_t hotRows,
                                            uint64_t overflowSlot)
 {
     if (slot < 0) return -1;
     const uint64_t row = b * reqStride + static_cast<uint32_t>(slot);
     if (row >= hotRows) {
-        if (overflowSlot != 0) {
-            // (the global address space: a flat access would have later LDS reads waited for in full)
-            typedef __attribute__((address_space(1))) unsigned long long Word;
-            unsigned long long none = 0;
-            __hip_atomic_compare_exchange_strong(reinterpret_cast<Word *>(overflowSlot), &none,
-                                                 static_cast<unsigned long long>(KVX_OVERFLOW_ROW), __ATOMIC_RELAXED,
-                                                 __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        }
+        report_row(overflowSlot);
         return -1;
     }
     return static_cast<int64_t>(row);

@@ -43,6 +43,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
     __shared__ float stat[kWaves][kRows][2], share[kWaves][kRows];
     static_assert(kWaves * kRows * kJoinStride * 4 <= kWaves * kTileBytes, "outputs fit the tiles");
 
+    take_arguments(a);
     const uint32_t lane = threadIdx.x & 63u;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t col = lane & 15u, grp = lane >> 4;
@@ -61,14 +62,12 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
         const uint32_t real = min(query, queries - 1);               // (what lies past the last query is not stored)
         const uint32_t node = real / a.heads, head = real % a.heads;
         const uint64_t at = a.q + req * a.qStrideB + node * a.qStrideT + head * a.qStrideH + grp * 16;
-#pragma unroll
-        for (int s = 0; s < kDim / 32; ++s) q[s] = *reinterpret_cast<const KVX_GLB u32x4 *>(at + s * 64);
+        // (before the queries: where it is not loaded the compiler waits for all loads)
         sees = a.treeMask != 0 ? reinterpret_cast<const KVX_GLB uint64_t *>(a.treeMask)[req * a.draft + node]
                                : ~0ull >> (63u - node);
-    }
-    const uint32_t flip = a.negate ? 0x80008000u : 0u;               // a negative scale: negative queries
 #pragma unroll
-    for (int s = 0; s < kDim / 32; ++s) q[s] ^= flip;
+        for (int s = 0; s < kDim / 32; ++s) q[s] = *reinterpret_cast<const KVX_GLB u32x4 *>(at + s * 64);
+    }
     float top = -INFINITY, sum = 0.0f;
     f32x4 o[kLatent / 16];
 #pragma unroll
@@ -162,6 +161,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
                 for (int n = 0; n < kPanels; ++n) loadPanel(panelAt(n));
             }
         }
+        have(q);
         for (uint32_t t = wave; t < chunk; t += kWaves) {
             const bool more = t + kWaves < chunk;
             const uint32_t live = static_cast<uint32_t>(__ballot(rowOf[t * kTile + (lane & 31u)] >= 0));
@@ -197,7 +197,11 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
                 sources(t + kWaves);
                 loadPanel(kFirst);
             }
-            if (live != ~0u || drafted) {
+            if (live != ~0u || drafted || a.negate != 0) {
+                if (a.negate != 0) {                 // a negative scale
+                    s[0] = -s[0];
+                    s[1] = -s[1];
+                }
                 const uint32_t selected = k0 >= a.topK ? 0u : (a.topK - k0 >= 32u ? ~0u : (1u << (a.topK - k0)) - 1u);
                 uint32_t own = 0;                    // drafted tokens' bits of this tile
                 if (drafted) own = static_cast<uint32_t>(k0 >= a.topK ? sees >> (k0 - a.topK) : sees << min(a.topK - k0, 63u));
@@ -325,6 +329,7 @@ template <int DTYPE>
 __global__ __launch_bounds__(kThreads) void kvx_tree_attention_join(AttnArgs a)
 {
     typedef typename Elem<DTYPE>::T T;
+    take_arguments(a);
     const uint32_t queries = a.draft * a.heads;
     const uint64_t row = static_cast<uint64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
     if (row >= static_cast<uint64_t>(a.reqs) * queries) return;

@@ -103,6 +103,15 @@ __device__ __forceinline__ float over_query(float x, F f)
 template <typename V>
 __device__ __forceinline__ void keep_in_acc(V &x) { asm volatile("" : "+a"(x)); }
 
+// The queries are there: without this the compiler waits for them, and so for
+// every load under way, at their first use in the loop over the tiles.
+template <int N>
+__device__ __forceinline__ void have(const u32x4 (&q)[N])
+{
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" ::"v"(q[i]));
+}
+
 // Byte of the 16-byte chunk c (0..7) of row r in a panel: rows one after
 // another are 128 bytes apart, so the chunks of 8 rows are permuted to spread a
 // column over the banks.
@@ -184,6 +193,17 @@ __device__ __forceinline__ void wait_panels(int n)
 
 // Every wave's LDS reads are done and what it waited for is there.
 __device__ __forceinline__ void meet() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// All of the arguments in scalar registers before anything else: each cache line
+// of them comes from far away (2000 to 2800 cycles), and the compiler would load
+// each where it is first used, one wait after another.
+__device__ __forceinline__ void take_arguments(const AttnArgs &a)
+{
+    asm volatile("" ::"s"(a.q), "s"(a.qStrideB), "s"(a.qStrideT), "s"(a.qStrideH), "s"(a.hot), "s"(a.hotRows),
+                 "s"(a.reqStride), "s"(a.slots), "s"(a.draftSlots), "s"(a.treeMask), "s"(a.out), "s"(a.lse));
+    asm volatile("" ::"s"(a.reqs), "s"(a.draft), "s"(a.heads), "s"(a.topK), "s"(a.scaleLog2), "s"(a.negate),
+                 "s"(a.overflowSlot), "s"(a.queryTiles), "s"(a.splits), "s"(a.part), "s"(a.partStat));
+}
 
 // The part of a call that a workgroup takes.  Consecutive parts go to one XCD
 // (workgroups go to the 8 XCDs in turn), so that the workgroups that read the

@@ -36,6 +36,14 @@ namespace {
 // r + 24 at once.
 __device__ __forceinline__ uint32_t chunk_in(uint32_t r, uint32_t c) { return chunk_at(r, c ^ (r >> 4)); }
 
+// A value that the compiler must not keep what it derives from it: addresses of
+// a lane that are cheaper made again than held in registers all the time.
+__device__ __forceinline__ uint32_t again(uint32_t x)
+{
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
 template <int LEFT>
 __device__ __forceinline__ void wait_loads_and_meet()
 {
@@ -73,7 +81,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
     constexpr int kKeySteps = kTile / (8 * G);       // ... output
     constexpr int kScores = kKeyTiles * kAcc;        // of a lane and tile: 8 or 16
     constexpr int kCols = kLatent / kRows;           // products over a row's columns
-    constexpr int kKeysAhead = 4 / kKeyTiles + 1, kColsAhead = 3 / kKeySteps + 1;   // operands read ahead
+    constexpr int kKeysAhead = 4 / kKeyTiles + (G == 4 ? 1 : 0), kValuesAhead = kCodes && G == 2 ? 3 : 4;        // operands read ahead
+    constexpr int kValues = kCols * kKeySteps;       // products of a tile's output
     // Buffers of whole tiles: the two worked on, and for 16-bit rows the two
     // under way; 8-bit rows arrive in buffers of their own and are converted
     // into a third.
@@ -86,6 +95,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
     __shared__ __align__(128) uint8_t tiles[kBuffers * kTileBytes + 2 * kRawBytes];
     __shared__ int32_t rowOf[kChunk * kTile];        // hot row within the request of each key, -1: none
 
+    take_arguments(a);
     const uint32_t lane = threadIdx.x & 63u;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t col = lane % kRows, grp = lane / kRows;
@@ -105,14 +115,12 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
         const uint32_t real = min(query, queries - 1);               // (what lies past the last query is not stored)
         const uint32_t node = real / a.heads, head = real % a.heads;
         const uint64_t at = a.q + req * a.qStrideB + node * a.qStrideT + head * a.qStrideH + grp * 16;
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s) q[s] = *reinterpret_cast<const KVX_GLB u32x4 *>(at + s * G * 16);
+        // (before the queries: where it is not loaded the compiler waits for all loads)
         sees = a.treeMask != 0 ? reinterpret_cast<const KVX_GLB uint64_t *>(a.treeMask)[req * a.draft + node]
                                : ~0ull >> (63u - node);
-    }
-    const uint32_t flip = a.negate ? 0x80008000u : 0u;               // a negative scale: negative queries
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) q[s] ^= flip;
+        for (int s = 0; s < kSteps; ++s) q[s] = *reinterpret_cast<const KVX_GLB u32x4 *>(at + s * G * 16);
+    }
     float top = -INFINITY, sum = 0.0f;
     Acc o[kCols];
 #pragma unroll
@@ -151,6 +159,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
         uint32_t to;
     };
     auto source = [&](uint32_t t, uint32_t n, uint32_t buffer) {
+        const uint32_t lane = again(threadIdx.x) & 63u;
         Source x;
         x.rows = rowStart(t, n, lane >> 3) + (kCodes ? lane & 7u : (lane & 7u) ^ (lane >> 3) ^ (wave >> 1)) * 16;
         x.scales = kRawScales != 0 ? rowStart(t, n, (lane >> 2) & 7u) + F::scaleAt + (lane & 3u) * 4 : nullptr;
@@ -166,6 +175,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
     u32x4 codes;
     uint32_t fourScales;
     auto readCodes = [&](uint32_t t, int p) {
+        const uint32_t lane = again(threadIdx.x) & 63u;
         const uint32_t raw = ldsRaw + (t & 1u) * kRawBytes;
         codes = *(const KVX_LDS u32x4 *)(uintptr_t)(raw + (p * 4 + wave) * 1024 + lane * 16);
         const uint32_t at = kRawScales != 0 ? raw + kTile * kRawPanels * 128 + wave * 256 + (lane >> 3) * 16 + p * 4
@@ -173,6 +183,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
         if (F::raw == 0 || p < 4) fourScales = *(const KVX_LDS uint32_t *)(uintptr_t)at;
     };
     auto writeValues = [&](uint32_t buffer, int p) {
+        const uint32_t lane = again(threadIdx.x) & 63u;
         const uint32_t r = wave * 8 + (lane >> 3), j = lane & 7u;
         const uint32_t to = ldsTiles + buffer + p * 2 * kPanelBytes;
         if (F::raw != 0 && p == 4) {
@@ -214,7 +225,11 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
     auto takeScores = [&](uint32_t live, uint32_t k0, bool drafted) {
 #pragma unroll
         for (int e = 0; e < kScores; ++e) c[e] = s[e / kAcc][e % kAcc];
-        if (live == ~0u && !drafted) return;
+        if (live == ~0u && !drafted && a.negate == 0) return;
+        if (a.negate != 0) {                         // a negative scale
+#pragma unroll
+            for (int e = 0; e < kScores; ++e) c[e] = -c[e];
+        }
         const uint32_t selected = k0 >= a.topK ? 0u : (a.topK - k0 >= 32u ? ~0u : (1u << (a.topK - k0)) - 1u);
         uint32_t own = 0;                            // drafted tokens' bits of this tile
         if (drafted) own = static_cast<uint32_t>(k0 >= a.topK ? sees >> (k0 - a.topK) : sees << min(a.topK - k0, 63u));
@@ -264,16 +279,14 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
 #pragma unroll
         for (int n = 0; n < kKeySteps; ++n) weight[n] = newWeight[n];
     };
-    u32x4 value[kColsAhead + 1][kKeySteps];
-    auto readColumns = [&](const KVX_LDS uint8_t *tile, int d) {
-#pragma unroll
-        for (int n = 0; n < kKeySteps; ++n) {
-            // keys 8 G n + 0.. and 8 G n + 4 G + 0..
-            auto at = [&](int k) { return (KVX_LDS s16x4 *)(tile + atValue[k / 16][d % G] + d / G * kPanelBytes + k % 16 * 128); };
-            const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at(8 * G * n));
-            const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at(8 * G * n + 4 * G));
-            value[d % (kColsAhead + 1)][n] = __builtin_bit_cast(u32x4, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
-        }
+    u32x4 value[kValuesAhead + 1];
+    auto readValue = [&](const KVX_LDS uint8_t *tile, int u) {
+        const int d = u / kKeySteps, n = u % kKeySteps;
+        // keys 8 G n + 0.. and 8 G n + 4 G + 0..
+        auto at = [&](int k) { return (KVX_LDS s16x4 *)(tile + atValue[k / 16][d % G] + d / G * kPanelBytes + k % 16 * 128); };
+        const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at(8 * G * n));
+        const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at(8 * G * n + 4 * G));
+        value[u % (kValuesAhead + 1)] = __builtin_bit_cast(u32x4, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
     };
 
     for (uint32_t c0 = item.tile0; c0 < item.tile1; c0 += kChunk) {
@@ -293,6 +306,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
                 const Source x = source(t, n, 0);
 #pragma unroll
                 for (int p = 0; p < kLoads; ++p) loadPart(x, p);
+                if (t == 0) have(q);
             }
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
@@ -313,6 +327,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
                 const Source x = source(t, n, t * kTileBytes);
 #pragma unroll
                 for (int p = 0; p < kLoads; ++p) loadPart(x, p);
+                if (t == 0) have(q);
             }
             wait_loads_and_meet<2 * kLoads>();
         }
@@ -364,13 +379,12 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
 #pragma unroll
                 for (int i = 0; i < kSteps; ++i) {
                     if (i + kKeysAhead < kSteps) readKeys(nextTile, i + kKeysAhead);
-                    if (i + kColsAhead >= kSteps) readColumns(tile, i + kColsAhead - kSteps);
+                    if (i + kValuesAhead >= kSteps) readValue(tile, i + kValuesAhead - kSteps);
                     if (i % (kSteps / 18) == 0) {    // (eighteenths of the way)
                         const int part = i / (kSteps / 18);
                         if (!kCodes && part % 2 == 0) loadPart(from, part / 2);
                         if (kCodes && part % 3 == 0 && part / 3 < kRawPanels) readCodes(t, part / 3);
                         if (kCodes && part % 3 == 2 && part / 3 < kRawPanels) writeValues(ahead(2), part / 3);
-                        if (kCodes && part == 16) from = source(t + 4, n, 0);
                     }
                     score(i);
                     __builtin_amdgcn_sched_barrier(0);
@@ -378,29 +392,28 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
                 takeScores(live, (c0 + t + 1) * kTile, isDrafted(t + 1));
             } else {
 #pragma unroll
-                for (int i = 0; i < kColsAhead; ++i) readColumns(tile, i);
+                for (int i = 0; i < kValuesAhead; ++i) readValue(tile, i);
 #pragma unroll
                 for (int p = 0; p < kLoads; ++p) {
                     if (!kCodes) loadPart(from, p);
                 }
             }
 #pragma unroll
-            for (int d = 0; d < kCols; ++d) {
-                if (d + kColsAhead < kCols) readColumns(tile, d + kColsAhead);
-                constexpr int kPart = kCols / 16;    // (sixteenths of the way)
-                if (d % kPart == 0) {
-                    const int part = d / kPart;
+            for (int u = 0; u < kValues; ++u) {
+                if (u + kValuesAhead < kValues) readValue(tile, u + kValuesAhead);
+                if (u % (kValues / 16) == 0) {       // (sixteenths of the way)
+                    const int part = u / (kValues / 16);
                     if (part < kScores / 8) lanesMost(part);
                     if (part == 2) decide();
 #pragma unroll
                     for (int e = (part - 3) * kScores / 12; part >= 3 && part < 15 && e < (part - 2) * kScores / 12; ++e) weigh(e);
                     if (kCodes && part >= 8) loadPart(from, part - 8);
+                    if (kCodes && part == 7) from = source(t + 4, n, 0);
                     // what the next round begins with
                     if (part == 3) live = liveKeys(min(t + 2, n - 1));
-                    if (!kCodes && part == 5) from = source(t + 4, n, buffer);
+                    if (!kCodes && part == 14) from = source(t + 4, n, buffer);
                 }
-#pragma unroll
-                for (int i = 0; i < kKeySteps; ++i) o[d] = P::mul(value[d % (kColsAhead + 1)][i], weight[i], o[d]);
+                o[u / kKeySteps] = P::mul(value[u % (kValuesAhead + 1)], weight[u % kKeySteps], o[u / kKeySteps]);
                 __builtin_amdgcn_sched_barrier(0);
             }
             if (more) settle();

@@ -40,7 +40,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
 
     __shared__ __align__(128) uint8_t tiles[kWaves * kTileBytes];    // and, at the end, the waves' outputs
     __shared__ int32_t rowOf[kChunk * kTile];        // hot row within the request of each key, -1: none
-    __shared__ float stat[kWaves][kRows][2], share[kWaves][kRows];
+    __shared__ float stat[kWaves][kRows][2];
+    __shared__ f32x4 share[kRows];                   // of the four waves
     static_assert(kWaves * kRows * kJoinStride * 4 <= kWaves * kTileBytes, "outputs fit the tiles");
 
     take_arguments(a);
@@ -287,23 +288,28 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
     for (int g = 0; g < kWaves; ++g) all += stat[g][col][1] * __builtin_amdgcn_exp2f(stat[g][col][0] - base);
     // ... and, where this is all of it, over the sum
     const float whole = a.splits > 1 ? 1.0f : (all == 0.0f ? 0.0f : __builtin_amdgcn_rcpf(all));
-    if (grp == 0) share[wave][col] = __builtin_amdgcn_exp2f(top - base) * whole;
+    if (grp == 0) reinterpret_cast<KVX_LDS float *>((KVX_LDS f32x4 *)&share[col])[wave] = __builtin_amdgcn_exp2f(top - base) * whole;
     KVX_LDS float *join = (KVX_LDS float *)tiles;
+    if (item.tile0 + wave < item.tile1) {
 #pragma unroll
-    for (int d = 0; d < kLatent / 16; ++d) {
-        keep_in_acc(o[d]);
-        *reinterpret_cast<KVX_LDS f32x4 *>(join + (wave * kRows + col) * kJoinStride + d * 16 + grp * 4) = o[d];
+        for (int d = 0; d < kLatent / 16; ++d) {
+            keep_in_acc(o[d]);
+            *reinterpret_cast<KVX_LDS f32x4 *>(join + (wave * kRows + col) * kJoinStride + d * 16 + grp * 4) = o[d];
+        }
     }
     __syncthreads();
     const uint64_t row0 = static_cast<uint64_t>(req) * queries;      // first output row of the request
     const uint64_t part0 = (static_cast<uint64_t>(req) * a.splits + item.split) * queries;
-#pragma unroll 2
-    for (int n = 0; n < kRows * (kLatent / 4) / kThreads; ++n) {
-        const uint32_t i = threadIdx.x + n * kThreads, c = i % (kLatent / 4), r = i / (kLatent / 4);
+    // (waves that had no tile have nothing to add)
+    const uint32_t busy = min(item.tile1 - item.tile0, static_cast<uint32_t>(kWaves));
+    const uint32_t c = threadIdx.x % (kLatent / 4);
+#pragma unroll 4
+    for (uint32_t r = threadIdx.x / (kLatent / 4); r < kRows; r += kThreads / (kLatent / 4)) {
+        const f32x4 part = share[r];
         f32x4 x = {};
 #pragma unroll
-        for (int g = 0; g < kWaves; ++g) {
-            x += *reinterpret_cast<const KVX_LDS f32x4 *>(join + (g * kRows + r) * kJoinStride + c * 4) * share[g][r];
+        for (uint32_t g = 0; g < kWaves; ++g) {
+            if (g < busy) x += *reinterpret_cast<const KVX_LDS f32x4 *>(join + (g * kRows + r) * kJoinStride + c * 4) * part[g];
         }
         const uint32_t index = item.queryTile * kRows + r;
         if (index >= queries) continue;
@@ -335,20 +341,36 @@ __global__ __launch_bounds__(kThreads) void kvx_tree_attention_join(AttnArgs a)
     if (row >= static_cast<uint64_t>(a.reqs) * queries) return;
     const uint32_t lane = threadIdx.x & 63u;
     const uint64_t first = row / queries * a.splits * queries + row % queries;
+    // a lane's split: its maximum and sum; then eight bytes of each split a lane, four splits under way
     const KVX_GLB f32x2 *stats = reinterpret_cast<const KVX_GLB f32x2 *>(a.partStat) + first;
-    float most = -INFINITY;
-    for (uint32_t s = 0; s < a.splits; ++s) most = fmaxf(most, stats[static_cast<uint64_t>(s) * queries].x);
+    f32x2 st = {-INFINITY, 0.0f};
+    if (lane < a.splits) st = stats[static_cast<uint64_t>(lane) * queries];
+    float most = st[0];
+#pragma unroll
+    for (int d = 32; d != 0; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
     const float base = most == -INFINITY ? 0.0f : most;
-    float all = 0.0f;
+    const float keep = __builtin_amdgcn_exp2f(st[0] - base);
+    float all = st[1] * keep;
+#pragma unroll
+    for (int d = 32; d != 0; d >>= 1) all += __shfl_xor(all, d);
     f32x4 x = {}, y = {};
-    for (uint32_t s = 0; s < a.splits; ++s) {
-        const uint64_t at = first + static_cast<uint64_t>(s) * queries;
-        const f32x2 st = stats[static_cast<uint64_t>(s) * queries];
-        const float keep = __builtin_amdgcn_exp2f(st.x - base);
-        all += st.y * keep;
-        const KVX_GLB f32x4 *v = reinterpret_cast<const KVX_GLB f32x4 *>(a.part) + at * (kLatent / 4) + lane * 2;
-        x += v[0] * keep;
-        y += v[1] * keep;
+    const KVX_GLB f32x4 *v = reinterpret_cast<const KVX_GLB f32x4 *>(a.part) + first * (kLatent / 4) + lane * 2;
+    const uint64_t step = static_cast<uint64_t>(queries) * (kLatent / 4);
+    for (uint32_t s = 0; s < a.splits; s += 4) {
+        f32x4 p[4][2];
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) {
+            const uint64_t at = min(s + j, a.splits - 1) * step;
+            p[j][0] = v[at];
+            p[j][1] = v[at + 1];
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) {
+            if (s + j >= a.splits) break;
+            const float k = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(keep), s + j));
+            x += p[j][0] * k;
+            y += p[j][1] * k;
+        }
     }
     const float inv = all == 0.0f ? 0.0f : __builtin_amdgcn_rcpf(all);
     *reinterpret_cast<KVX_GLB u32x4 *>(reinterpret_cast<KVX_GLB T *>(a.out) + row * kLatent + lane * 8) =

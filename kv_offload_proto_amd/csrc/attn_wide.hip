@@ -81,7 +81,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
     constexpr int kKeySteps = kTile / (8 * G);       // ... output
     constexpr int kScores = kKeyTiles * kAcc;        // of a lane and tile: 8 or 16
     constexpr int kCols = kLatent / kRows;           // products over a row's columns
-    constexpr int kKeysAhead = 4 / kKeyTiles + (G == 4 ? 1 : 0), kValuesAhead = kCodes && G == 2 ? 3 : 4;        // operands read ahead
+    constexpr int kKeysAhead = G == 4 ? 6 : 4, kValuesAhead = G == 4 ? 10 : (kCodes ? 3 : 4);   // operands read ahead
     constexpr int kValues = kCols * kKeySteps;       // products of a tile's output
     // Buffers of whole tiles: the two worked on, and for 16-bit rows the two
     // under way; 8-bit rows arrive in buffers of their own and are converted

@@ -66,13 +66,24 @@ int kvx_dequantize_rows(uint64_t hot_row_base, uint64_t hot_rows, uint64_t slots
  *   out[b][t][h] = sum exp(s - lse) * first 512 values  (dtype, contiguous)
  * and zeros with lse -inf where a query sees no key.  A key listed twice
  * counts twice.  What rows hold that a query does not see has no effect on it,
- * NaN and infinities included.  draft <= 64, heads <= 1024.  Scores, sums and the output
- * are accumulated in 32 bits, the weights exp(s - max) rounded to dtype. */
+ * NaN and infinities included.  draft <= 64, heads <= 1024, softmax_scale
+ * finite.  Scores, sums and the output are accumulated in 32 bits, the weights
+ * exp(s - max) rounded to dtype (fp16 weights below 2^-24 of a query's largest
+ * can be lost).
+ * A call that needs scratch takes it from its stream's; to record one into a
+ * graph, size it first with kvx_reserve_attention. */
 int kvx_tree_attention(uint64_t q, uint64_t q_stride_b, uint64_t q_stride_t, uint64_t q_stride_h,
                        uint64_t hot_row_base, uint64_t hot_rows, uint64_t slots, uint64_t draft_slots,
                        uint64_t tree_mask, uint64_t out, uint64_t lse, uint32_t num_reqs, uint32_t draft,
                        uint32_t heads, uint32_t top_k, uint64_t req_stride_rows, float softmax_scale,
                        uint32_t kv_lora_rank, uint32_t qk_rope, uint32_t dtype, uint32_t quant, uint64_t stream);
+
+/* Allocate the scratch that calls of exactly these sizes use on `stream`
+ * (drafted: nonzero where draft_slots is given; quant: the form of the rows),
+ * so that they can be captured there.  A stream keeps the most it was ever
+ * asked for (kvx_scratch_bytes). */
+int kvx_reserve_attention(uint64_t stream, uint32_t num_reqs, uint32_t draft, uint32_t heads, uint32_t top_k,
+                          uint32_t drafted, uint32_t quant);
 
 #ifdef __cplusplus
 }

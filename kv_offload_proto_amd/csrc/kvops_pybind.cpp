@@ -281,6 +281,12 @@ PYBIND11_MODULE(_kvops, m)
         py::arg("req_stride_rows"), py::arg("dst"), py::arg("kv_lora_rank"), py::arg("qk_rope"), py::arg("dtype"),
         py::arg("quant"), py::arg("out_dtype"), py::arg("stream") = 0);
     m.def(
+        "reserve_attention",
+        [](uint64_t stream, uint32_t num_reqs, uint32_t draft, uint32_t heads, uint32_t top_k, uint32_t drafted,
+           uint32_t quant) { Check(kvx_reserve_attention(stream, num_reqs, draft, heads, top_k, drafted, quant)); },
+        py::arg("stream"), py::arg("num_reqs"), py::arg("draft"), py::arg("heads"), py::arg("top_k"),
+        py::arg("drafted"), py::arg("quant"));
+    m.def(
         "tree_attention",
         [](uint64_t q, uint64_t q_stride_b, uint64_t q_stride_t, uint64_t q_stride_h, uint64_t hot_row_base,
            uint64_t hot_rows, uint64_t slots, uint64_t draft_slots, uint64_t tree_mask, uint64_t out, uint64_t lse,

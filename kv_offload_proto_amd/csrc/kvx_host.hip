@@ -228,8 +228,8 @@ void *ScratchAlloc(uint64_t bytes, hipStream_t stream, const char *what)
 
 // The scratch of `stream`, created or grown to `need`.  Creation and growth
 // allocate and queue a clear on the stream; both are refused while the stream
-// is being captured (kvx_reserve_scratch sizes a stream beforehand).  The
-// caller holds g_scratchMu.
+// is being captured (kvx_reserve_scratch and kvx_reserve_attention size a
+// stream beforehand).  The caller holds g_scratchMu.
 StreamScratch &ScratchFor(uint64_t stream, const ScratchNeed &need, const char *what)
 {
     StreamScratch *sc = nullptr;
@@ -243,7 +243,8 @@ StreamScratch &ScratchFor(uint64_t stream, const ScratchNeed &need, const char *
     hipStream_t st = AsStream(stream);
     if (Capturing(st)) {
         throw Error(std::string(what) + ": the scratch of this stream is too small for the call and cannot grow "
-                    "during stream capture; call reserve_scratch for the stream before capturing");
+                    "during stream capture; call " +
+                    (need.attn != 0 ? "reserve_attention" : "reserve_scratch") + " for the stream before capturing");
     }
     if (create) {
         auto *s = new StreamScratch();
@@ -509,6 +510,16 @@ void CheckRowForm(const char *what, uint32_t latent, uint32_t rope, uint32_t dty
     if (dtype > KVX_DTYPE_FP16) throw Error(std::string(what) + ": dtype must be bf16 or fp16");
     if (quant > KVX_QUANT_ROW) throw Error(std::string(what) + ": unknown row form");
     if (codes && quant == KVX_QUANT_NONE) throw Error(std::string(what) + ": rows of 16-bit values hold no codes");
+}
+
+void CheckAttnSizes(const char *what, uint32_t num_reqs, uint32_t draft, uint32_t heads, uint32_t top_k)
+{
+    if (draft > 64) throw Error(std::string(what) + ": draft must be <= 64");
+    if (heads > 1024) throw Error(std::string(what) + ": heads must be <= 1024");
+    if (top_k > (1u << 30)) throw Error(std::string(what) + ": top_k must be <= 2^30");
+    if (static_cast<uint64_t>(num_reqs) * draft * heads >= 1ull << 31) {
+        throw Error(std::string(what) + ": num_reqs * draft * heads must be below 2^31");
+    }
 }
 
 kvx::RowCopyArgs RowCopy(const char *what, uint64_t rows16, uint64_t rowStride, uint64_t hot, uint64_t hotRows,
@@ -1195,6 +1206,22 @@ int kvx_dequantize_rows(uint64_t hot_row_base, uint64_t hot_rows, uint64_t slots
     });
 }
 
+int kvx_reserve_attention(uint64_t stream, uint32_t num_reqs, uint32_t draft, uint32_t heads, uint32_t top_k,
+                          uint32_t drafted, uint32_t quant)
+{
+    return Guarded([&] {
+        EnsureInited();
+        if (quant > KVX_QUANT_ROW) throw Error("reserve_attention: unknown quant");
+        CheckAttnSizes("reserve_attention", num_reqs, draft, heads, top_k);
+        if (num_reqs == 0 || draft == 0 || heads == 0) return;
+        ScratchNeed need;
+        need.attn = kvx::plan_tree_attention(num_reqs, draft, heads, top_k, drafted != 0, quant != KVX_QUANT_NONE).floats;
+        if (need.attn == 0) return;
+        std::lock_guard<std::mutex> lk(g_scratchMu);
+        (void)ScratchFor(stream, need, "reserve_attention");
+    });
+}
+
 int kvx_tree_attention(uint64_t q, uint64_t q_stride_b, uint64_t q_stride_t, uint64_t q_stride_h,
                        uint64_t hot_row_base, uint64_t hot_rows, uint64_t slots, uint64_t draft_slots,
                        uint64_t tree_mask, uint64_t out, uint64_t lse, uint32_t num_reqs, uint32_t draft,
@@ -1204,10 +1231,9 @@ int kvx_tree_attention(uint64_t q, uint64_t q_stride_b, uint64_t q_stride_t, uin
     return Guarded([&] {
         EnsureInited();
         CheckRowForm("tree_attention", kv_lora_rank, qk_rope, dtype, quant, false);
+        CheckAttnSizes("tree_attention", num_reqs, draft, heads, top_k);
         if (num_reqs == 0 || draft == 0 || heads == 0) return;
-        if (draft > 64) throw Error("tree_attention: draft must be <= 64");
-        if (heads > 1024) throw Error("tree_attention: heads must be <= 1024");
-        if (top_k > (1u << 30)) throw Error("tree_attention: top_k must be <= 2^30");
+        if (!std::isfinite(softmax_scale)) throw Error("tree_attention: softmax_scale must be finite");
         CheckAligned16(q, "tree_attention: q");
         CheckAligned16(hot_row_base, "tree_attention: hot_row_base");
         CheckAligned16(out, "tree_attention: out");
@@ -1239,9 +1265,6 @@ int kvx_tree_attention(uint64_t q, uint64_t q_stride_b, uint64_t q_stride_t, uin
         a.scaleLog2 = std::max(std::fabs(softmax_scale) * 1.4426950408889634f, 1e-30f);
         a.negate = softmax_scale < 0.0f ? 1u : 0u;
         a.overflowSlot = reinterpret_cast<uint64_t>(g.overflow);
-        if (static_cast<uint64_t>(num_reqs) * draft * heads >= 1ull << 31) {
-            throw Error("tree_attention: num_reqs * draft * heads must be below 2^31");
-        }
         const kvx::AttnPlan p = kvx::plan_tree_attention(num_reqs, draft, heads, top_k, draft_slots != 0,
                                                           quant != KVX_QUANT_NONE);
         float *scratch = nullptr;

@@ -15,7 +15,8 @@ layer with 8-bit rows:
                               draft_slots=new_slots, tree_mask=mask)
 
 Everything is asynchronous on torch's current stream unless a stream is given,
-and can be recorded into a graph.  The reference has no counterpart: it moves
+and can be recorded into a graph (``reserve_attention`` first, on the stream
+that captures).  The reference has no counterpart: it moves
 rows as bytes.
 """
 from functools import lru_cache
@@ -221,3 +222,15 @@ def tree_attention(fmt: RowFormat, q: torch.Tensor, hot: torch.Tensor, slots: to
                           out.data_ptr(), lse.data_ptr(), reqs, tokens, heads, slots.shape[1],
                           req_stride_rows, softmax_scale, *fmt.code, _stream_of(stream, device))
     return out, lse
+
+
+def reserve_attention(fmt: RowFormat, requests: int, tokens: int, heads: int, top_k: int, drafted: bool = False,
+                      stream=None) -> None:
+    """Allocate what ``tree_attention`` calls of these sizes keep on the stream
+    (default: the current one), so that a graph can capture them there;
+    ``drafted``: with ``draft_slots``.  Replays use the capture stream's
+    scratch and must not overlap each other or other calls on that stream."""
+    if min(requests, tokens, heads, top_k) < 0:
+        raise ValueError("sizes must not be negative")
+    _kvops.reserve_attention(_stream_of(stream, torch.cuda.current_device()), requests, tokens, heads, top_k,
+                             int(drafted), fmt.code[3])

@@ -7,9 +7,11 @@
 // waits for another wave until their outputs are joined at the end.  The tile
 // that a wave loads next replaces the one it works on panel by panel, as the
 // output's products are done with each, so that a load is under way nearly all
-// the time; memory bounds this kernel, or, where several workgroups read the
-// same keys, the way from L2 to LDS (64 bytes a cycle: a wave's tile 576 cycles,
-// while the matrix unit needs 1088 and works for four waves at once).
+// the time.  Memory bounds this kernel where there are many requests (64 of 16
+// queries and 2048 keys in 8 bits: 25 us for 104 MB, 4.2 TB/s), or, where several
+// workgroups read the same keys, the way from L2 to LDS (12 TB/s measured: 16
+// queries a workgroup, 128 a request: 107 us).  A call of one tile takes 8 us:
+// launch, arguments, slots, rows and the joining of the waves one after another.
 //
 // Scores are held transposed, S^T = K Q^T (keys down, queries across the
 // lanes), so that a lane's scores, its running maximum and its sum all belong
@@ -392,11 +394,18 @@ void launch(const AttnArgs &a, hipStream_t stream)
 // Queries a workgroup and workgroups that share a query's keys, by the time that
 // each way is expected to take: a workgroup's start and end, its tiles one after
 // another (16 queries: four at a time), as many rounds of workgroups as the 256
-// CUs need, and the joining.  The figures are microseconds measured on an MI355X
-// with all CUs at work; what they decide, measured both ways (us):
-//   64 requests x 128 queries, 2048 keys: 16 wide 101, 64 in 2 splits 75, 128 in 4 splits 81
-//   4 x 4096 queries, 8192 keys: 16 wide 587, 64 wide 373, 128 in 2 splits 316
-//   1 x 256 queries, 2048 keys: 16 in 8 splits 21, 64 in 16 splits 29, 128 in 16 splits 39
+// CUs need, and the joining (a launch, and the outputs written and read again).
+// The figures are microseconds of an MI355X with all CUs at work.  What they
+// decide, us a call measured both ways, the rule's choice first:
+//   64 requests x 128 queries, 2048 keys     64 wide in 2 splits 63, 128 in 4: 68, 16: 107
+//   ... in 8 bits                            128 in 4 splits 72, 64 in 2: 82, 16: 95
+//   64 x 16 queries, 2048 keys in 8 bits     16 in 4 splits 29, in 2: 34, in 8: 40, alone: 44
+//   4 x 4096 queries, 8224 keys              128 in 2 splits 285, 64: 318, 16: 551
+//   16 x 1024 queries, 2056 keys in 8 bits   128 in 2 splits 115, 64: 134, 16: 191
+//   1 x 256 queries, 2050 keys               16 in 8 splits 19, 64 in 16: 24, 128 in 16: 31
+//   8 x 16 queries, 64 keys                  16 alone 8.2, in 2 splits 11.0
+// Not more than 1024 workgroups share keys: more would be rounds after another
+// that the joining adds to.
 AttnPlan plan_tree_attention(uint32_t reqs, uint32_t draft, uint32_t heads, uint32_t topK, bool drafted, bool codes)
 {
     struct Width {

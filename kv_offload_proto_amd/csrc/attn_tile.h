@@ -232,8 +232,9 @@ struct AttnItem {
 };
 
 // The slots of n tiles from c0 on into LDS, -1 where they name no row.  Four at
-// a time, and no more code than that: what a launch runs once it waits for,
-// about a microsecond for each 2 KB of instructions.
+// a time, and no more code than that: code that a workgroup runs once is fetched
+// while it waits (eight at a time, 64-bit compares and a report each: 1 to 2 us
+// more a call).
 __device__ __forceinline__ void look_up(const AttnArgs &a, const AttnItem &item, uint32_t c0, uint32_t n, int32_t *rowOf)
 {
     const KVX_GLB int32_t *selected = reinterpret_cast<const KVX_GLB int32_t *>(a.slots) + static_cast<uint64_t>(item.req) * a.topK;

@@ -49,7 +49,10 @@ def parse_args(argv=None):
     p.add_argument("--steps", type=int, default=10)
     p.add_argument("--seed", type=int, default=42)
     p.add_argument("--no-check", action="store_true")
-    return p.parse_args(argv)
+    args = p.parse_args(argv)
+    if not 1 <= args.draft <= 64:
+        p.error("--draft must be in [1, 64]")
+    return args
 
 
 def draw_tree(rng, reqs, tokens):

@@ -54,6 +54,9 @@ CASES = [
     (5, 50, 60, 2200, 2300, "bf16", "none", True, 0),
     (5, 64, 64, 2500, 2600, "fp16", "none", True, 0),
     (3, 64, 128, 150, 160, "fp16", "latent", True, 0),
+    (4, 32, 128, 1500, 1600, "bf16", "none", True, 0.01),
+    (16, 8, 127, 1200, 1300, "fp16", "none", True, 0),
+    (8, 16, 128, 1400, 1410, "bf16", "row", False, 0),
 ]
 
 

@@ -146,10 +146,12 @@ def dequantize_rows(fmt: RowFormat, hot: torch.Tensor, slots: Optional[torch.Ten
                     stream=None) -> torch.Tensor:
     """The values of the hot rows that ``slots`` (int32 [requests, rows of
     each]) name, as [requests * rows, dim] of ``dtype`` (default ``fmt.dtype``;
-    any 16-bit float or float32); zeros where a slot is negative.  Without
+    bfloat16, float16 or float32); zeros where a slot is negative.  Without
     slots: of every hot row (as many as ``out`` has, where it is given)."""
     _needs_codes(fmt)
     hot_rows = _hot(fmt, hot)
+    if dtype is not None and dtype not in _DTYPES:
+        raise ValueError("dtype must be bfloat16, float16 or float32, got {}".format(dtype))
     if out is None:
         n = hot_rows if slots is None else slots.numel()
         out = torch.empty((n, fmt.dim), dtype=dtype or fmt.dtype, device=hot.device)

@@ -8,7 +8,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_gpu_attention import dev, problem, run
+from test_gpu_attention import check, dev, problem, run
 
 pytestmark = pytest.mark.gpu
 
@@ -114,6 +114,21 @@ def test_reserve_grows_once(kvops):
 def test_scale_that_is_not_finite_is_refused(scale):
     with pytest.raises(RuntimeError, match="softmax_scale must be finite"):
         run(problem(1, 1, 2, 4, 8, "bf16", "row", False), scale=scale)
+
+
+@pytest.mark.parametrize("heads,dtype,quant", [(3, "bf16", "none"), (150, "fp16", "row")])
+def test_scale_of_zero_weighs_all_alike(heads, dtype, quant):
+    p = problem(2, 3, heads, 70, 90, dtype, quant, True, holes=0.2)
+    check(p, *run(p, scale=0.0), scale=0.0)
+
+
+@pytest.mark.parametrize("dtype", [torch.float64, torch.int16])
+def test_values_of_another_type_are_refused(dtype):
+    from kv_offload_proto_amd import xds
+
+    fmt = xds.row_format(torch.bfloat16, quant="row")
+    with pytest.raises(ValueError, match="dtype must be"):
+        xds.dequantize_rows(fmt, torch.zeros((4, fmt.row_bytes), dtype=torch.uint8, device="cuda"), dtype=dtype)
 
 
 @pytest.mark.parametrize("flags", [

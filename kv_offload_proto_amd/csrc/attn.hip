@@ -393,16 +393,20 @@ void launch(const AttnArgs &a, hipStream_t stream)
 
 // Queries a workgroup and workgroups that share a query's keys, by the time that
 // each way is expected to take: a workgroup's start and end, its tiles one after
-// another (16 queries: four at a time), as many rounds of workgroups as the 256
-// CUs need, and the joining (a launch, and the outputs written and read again).
-// The figures are microseconds of an MI355X with all CUs at work.  What they
-// decide, us a call measured both ways, the rule's choice first:
-//   64 requests x 128 queries, 2048 keys     64 wide in 2 splits 63, 128 in 4: 68, 16: 107
+// another (16 queries: four at a time), which take longer as more of the 256 CUs
+// are at work, as many rounds of workgroups as the CUs need, and the joining: a
+// launch, the splits one after another, and the outputs written and read again.
+// The figures are microseconds fitted to an MI355X.  What they decide, us a call
+// measured both ways, the rule's choice first:
+//   64 requests x 128 queries, 2048 keys     64 wide in 2 splits 62, 128 in 4: 68, 16: 107
 //   ... in 8 bits                            128 in 4 splits 72, 64 in 2: 82, 16: 95
+//   32 x 128 queries, 2048 keys              64 wide in 4 splits 40, 16: 46, 128 in 6: 49
 //   64 x 16 queries, 2048 keys in 8 bits     16 in 4 splits 29, in 2: 34, in 8: 40, alone: 44
+//   8 x 16 queries, 2048 keys                16 in 8 splits 18.5, in 4: 21, in 16: 20.5
+//   1 x 16 queries, 8192 keys                16 in 22 splits 24, in 8: 29, in 64: 33
 //   4 x 4096 queries, 8224 keys              128 in 2 splits 285, 64: 318, 16: 551
 //   16 x 1024 queries, 2056 keys in 8 bits   128 in 2 splits 115, 64: 134, 16: 191
-//   1 x 256 queries, 2050 keys               16 in 8 splits 19, 64 in 16: 24, 128 in 16: 31
+//   1 x 256 queries, 2050 keys               16 in 9 splits 19, 64 in 16: 24, 128 in 16: 31
 //   8 x 16 queries, 64 keys                  16 alone 8.2, in 2 splits 11.0
 // Not more than 1024 workgroups share keys: more would be rounds after another
 // that the joining adds to.
@@ -410,9 +414,12 @@ AttnPlan plan_tree_attention(uint32_t reqs, uint32_t draft, uint32_t heads, uint
 {
     struct Width {
         uint32_t rows, atOnce;
-        float ends, tiles16, tiles8;     // of 16-bit and of 8-bit rows
+        float ends;
+        float tiles16, busy16, tiles8, busy8;        // of 16-bit and of 8-bit rows: few workgroups, added with all
     };
-    constexpr Width widths[] = {{16, 4, 9.5f, 1.8f, 2.3f}, {64, 1, 12.0f, 1.42f, 1.85f}, {128, 1, 15.0f, 2.15f, 2.55f}};
+    constexpr Width widths[] = {{16, 4, 9.1f, 1.75f, 0.45f, 2.0f, 0.6f},
+                                {64, 1, 9.5f, 1.1f, 0.12f, 1.55f, 0.2f},
+                                {128, 1, 12.0f, 1.6f, 0.35f, 1.9f, 0.4f}};
     const uint32_t queries = draft * heads;
     const uint32_t tiles = std::max(1u, (topK + (drafted ? draft : 0u) + kTile - 1) / kTile);
     AttnPlan p{};
@@ -420,13 +427,15 @@ AttnPlan plan_tree_attention(uint32_t reqs, uint32_t draft, uint32_t heads, uint
     for (const Width &w : widths) {
         const uint32_t queryTiles = (queries + w.rows - 1) / w.rows;
         if (w.rows > 16 && queries <= w.rows / 4) break;       // (mostly empty)
-        for (uint32_t splits = 1; splits <= std::min(tiles, 64u); splits += splits < 4 ? 1 : splits / 2) {
+        for (uint32_t n = 1; n <= std::min(tiles, 64u); n += n < 4 ? 1 : n / 2) {
+            const uint32_t steps = ((tiles + n - 1) / n + w.atOnce - 1) / w.atOnce;
+            const uint32_t splits = (tiles + steps * w.atOnce - 1) / (steps * w.atOnce);     // (no more than that takes)
             const uint64_t items = static_cast<uint64_t>(reqs) * queryTiles * splits;
             if (splits > 1 && items > 1024) break;
-            const uint32_t steps = ((tiles + splits - 1) / splits + w.atOnce - 1) / w.atOnce;
             const float rounds = static_cast<float>((items + 255) / 256);
-            float us = (w.ends + steps * (codes ? w.tiles8 : w.tiles16)) * rounds;
-            if (splits > 1) us += 5.0f + static_cast<float>(reqs) * queries * splits * (kLatent * 4) * 0.3e-6f;
+            const float busy = std::min(static_cast<float>(items) / 256.0f, 1.0f);
+            float us = (w.ends + steps * (codes ? w.tiles8 + w.busy8 * busy * busy : w.tiles16 + w.busy16 * busy * busy)) * rounds;
+            if (splits > 1) us += 3.0f + 0.3f * splits + static_cast<float>(reqs) * queries * splits * (kLatent * 4) * 0.3e-6f;
             if (p.rows == 0 || us < best) {
                 best = us;
                 p.rows = w.rows;

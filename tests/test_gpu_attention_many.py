@@ -57,6 +57,8 @@ CASES = [
     (4, 32, 128, 1500, 1600, "bf16", "none", True, 0.01),
     (16, 8, 127, 1200, 1300, "fp16", "none", True, 0),
     (8, 16, 128, 1400, 1410, "bf16", "row", False, 0),
+    (32, 1, 128, 1100, 1200, "fp16", "none", False, 0.05),
+    (4, 32, 128, 4200, 4300, "bf16", "none", True, 0),
 ]
 
 

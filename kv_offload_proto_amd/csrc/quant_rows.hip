@@ -26,6 +26,7 @@ constexpr int kUnitsPerLane = kRowsPerBlock * kUnits / kThreads;
 static_assert(kRowsPerBlock * kUnits == kThreads * kUnitsPerLane, "whole units a lane");
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef u32x4 u32x4_8 __attribute__((aligned(8)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -160,12 +161,13 @@ __global__ __launch_bounds__(kThreads) void kvx_dequantize_rows(RowCopyArgs a)
         x[i] = u32x4{0, 0, 0, 0};
         if (from[r] >= 0) {
             const uint64_t src = a.hot + static_cast<uint64_t>(from[r]) * F::bytes;
-            if (F::raw == 0 || c < F::codes / 8) {
+            if constexpr (F::raw == 0) {
                 const u32x2 codes = *reinterpret_cast<const KVX_GLB u32x2 *>(src + c * 8);
                 x[i][0] = codes[0];
                 x[i][1] = codes[1];
             } else {
-                x[i] = *reinterpret_cast<const KVX_GLB u32x4 *>(src + F::codes + (c - F::codes / 8) * 16);
+                // 16 bytes in any case: two kinds of loads would wait for each other (2.7 TB/s, not 5)
+                x[i] = *reinterpret_cast<const KVX_GLB u32x4_8 *>(src + (c < F::codes / 8 ? c * 8 : F::codes + (c - F::codes / 8) * 16));
             }
         }
     }
@@ -183,25 +185,26 @@ __global__ __launch_bounds__(kThreads) void kvx_dequantize_rows(RowCopyArgs a)
     for (int i = 0; i < 2 * kUnitsPerLane; ++i) {
         const uint32_t u = threadIdx.x + i * kThreads, r = u / (2 * kUnits), c = u % (2 * kUnits);
         if (row0 + r >= a.rows) continue;
+        // Both ways and a choice, not a branch: a store in each half of a branch
+        // halved the rate of rows whose rotary part is copied.
+        const bool code = F::raw == 0 || c < F::codes / 8;
+        const uint32_t byte = scales[r][code ? c / 4 : 0];
+        const float scale = __uint_as_float(byte == 0 ? 0x00400000u : byte << 23);      // (2^-127 has no normal form)
         float v[8];
-        if (F::raw == 0 || c < F::codes / 8) {
-            // 2^-127 has no normal form
-            const uint32_t byte = scales[r][c / 4];
-            const float scale = __uint_as_float(byte == 0 ? 0x00400000u : byte << 23);
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(x[i][j]), false);
-                const f32x2 hi = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(x[i][j]), true);
-                v[4 * j] = lo[0] * scale;
-                v[4 * j + 1] = lo[1] * scale;
-                v[4 * j + 2] = hi[0] * scale;
-                v[4 * j + 3] = hi[1] * scale;
-            }
-        } else {
+        for (int j = 0; j < 2; ++j) {
+            const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(x[i][j]), false);
+            const f32x2 hi = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(x[i][j]), true);
+            v[4 * j] = lo[0] * scale;
+            v[4 * j + 1] = lo[1] * scale;
+            v[4 * j + 2] = hi[0] * scale;
+            v[4 * j + 3] = hi[1] * scale;
+        }
+        if (F::raw != 0 && OUT != DTYPE) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                v[2 * j] = to_float<DTYPE>(x[i][j] & 0xFFFFu);
-                v[2 * j + 1] = to_float<DTYPE>(x[i][j] >> 16);
+                v[2 * j] = code ? v[2 * j] : to_float<DTYPE>(x[i][j] & 0xFFFFu);
+                v[2 * j + 1] = code ? v[2 * j + 1] : to_float<DTYPE>(x[i][j] >> 16);
             }
         }
         const uint64_t at = (row0 + r) * kDim + c * 8;
@@ -210,8 +213,12 @@ __global__ __launch_bounds__(kThreads) void kvx_dequantize_rows(RowCopyArgs a)
             out[0] = f32x4{v[0], v[1], v[2], v[3]};
             out[1] = f32x4{v[4], v[5], v[6], v[7]};
         } else {
-            __builtin_nontemporal_store(u32x4{pack2<OUT>(v[0], v[1]), pack2<OUT>(v[2], v[3]), pack2<OUT>(v[4], v[5]), pack2<OUT>(v[6], v[7])},
-                                        reinterpret_cast<KVX_GLB u32x4 *>(a.rows16 + at * 2));
+            u32x4 y = {pack2<OUT>(v[0], v[1]), pack2<OUT>(v[2], v[3]), pack2<OUT>(v[4], v[5]), pack2<OUT>(v[6], v[7])};
+            if (F::raw != 0 && OUT == DTYPE) {       // (as they are)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) y[j] = code ? y[j] : x[i][j];
+            }
+            __builtin_nontemporal_store(y, reinterpret_cast<KVX_GLB u32x4 *>(a.rows16 + at * 2));
         }
     }
 }
